@@ -62,6 +62,19 @@ int getmi_scale_cast_impl(const float*, const float*, int, bf16_t*, float*, int,
 size_t getmi_scale_cast_noalloc_max_bytes_impl(void);
 int getmi_scale_cast_noalloc_impl(const float*, const float*, int, bf16_t*, float*, int, int, int, hipStream_t);
 
+int getmi_rmsnorm_fwd_impl(const void*, int, int64_t, const void*, int, int64_t, const float*, void*, int, void*, float*, int, int, float,
+                           hipStream_t);
+int getmi_rmsnorm_fp8_impl(const void*, int, int64_t, const void*, int, int64_t, const float*, void*, void*, int, void*, int, int, float,
+                           hipStream_t);
+size_t getmi_rmsnorm_bwd_workspace_bytes_impl(int M, int D);
+int getmi_rmsnorm_bwd_impl(const void*, int, const void*, int, int64_t, const float*, const float*, const void*, void*, void*, float*, int,
+                           int, void*, size_t, hipStream_t);
+int getmi_quant_blocks_fp8_impl(const void*, int, int64_t, void*, void*, int, int, int, hipStream_t);
+int getmi_gemm_fp8_impl(const void*, const void*, const void*, const void*, const float*, void*, int, int, int, int64_t, int64_t, int64_t,
+                        int, int, hipStream_t);
+int getmi_rotary_impl(const void*, void*, int, const void*, void*, int, const int64_t*, int, int, int, int, int, const double*, const void*,
+                      int, int64_t, int64_t, int64_t, int, int, float, hipStream_t);
+
 struct AdamGroup { float lr, weight_decay, beta1, beta2, eps, step_size, inv_sqrt_bc2, pad; };
 int getmi_adamw_step_impl(const void* jobs, int nflat, int ntile, const AdamGroup* groups, int ngroups, hipStream_t st);
 
@@ -220,6 +233,33 @@ int getmi_gemm_wgrad_pair(const void* Xa, const void* Ya, int N1a, int N2a, int 
                                       ldyb, outb, accumulate_b, M, reinterpret_cast<float*>(workspace), workspace_bytes,
                                       ST(stream));
 }
+int getmi_rmsnorm_fwd(const void* x, int x_type, int64_t ldx, const void* residual, int residual_type, int64_t ldr, const float* w, void* y,
+                      int y_type, void* h, float* rstd, int M, int D, float eps, void* stream) {
+    return getmi_rmsnorm_fwd_impl(x, x_type, ldx, residual, residual_type, ldr, w, y, y_type, h, rstd, M, D, eps, ST(stream));
+}
+int getmi_rmsnorm_fp8(const void* x, int x_type, int64_t ldx, const void* residual, int residual_type, int64_t ldr, const float* w, void* q,
+                      void* scales, int lds, void* h, int M, int D, float eps, void* stream) {
+    return getmi_rmsnorm_fp8_impl(x, x_type, ldx, residual, residual_type, ldr, w, q, scales, lds, h, M, D, eps, ST(stream));
+}
+size_t getmi_rmsnorm_bwd_workspace_bytes(int M, int D) { return getmi_rmsnorm_bwd_workspace_bytes_impl(M, D); }
+int getmi_rmsnorm_bwd(const void* dy, int dy_type, const void* h, int h_type, int64_t ldh, const float* rstd, const float* w, const void* dh,
+                      void* dx, void* dx2, float* dw, int M, int D, void* workspace, size_t workspace_bytes, void* stream) {
+    return getmi_rmsnorm_bwd_impl(dy, dy_type, h, h_type, ldh, rstd, w, dh, dx, dx2, dw, M, D, workspace, workspace_bytes, ST(stream));
+}
+int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void* scales, int lds, int N, int K, void* stream) {
+    return getmi_quant_blocks_fp8_impl(w, w_type, ldw, q, scales, lds, N, K, ST(stream));
+}
+int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
+                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream) {
+    return getmi_gemm_fp8_impl(A, sa, B, sb, bias, out, M, N, K, lda, ldb, ldo, lsa, lsb, ST(stream));
+}
+int getmi_rotary(const void* q, void* qo, int hq, const void* k, void* ko, int hk, const int64_t* strides, int type, int B, int T, int D,
+                 int R, const double* inv_freq, const void* pos, int pos64, int64_t pb, int64_t pt, int64_t offset, int interleaved,
+                 int backward, float magnitude, void* stream) {
+    return getmi_rotary_impl(q, qo, hq, k, ko, hk, strides, type, B, T, D, R, inv_freq, pos, pos64, pb, pt, offset, interleaved, backward,
+                             magnitude, ST(stream));
+}
+
 int getmi_set_cu_limit(int n) { return getmi_set_cu_limit_impl(n); }
 int getmi_cu_count(void) { return getmi_cu_count_impl(); }
 

@@ -14,10 +14,12 @@ Granularity follows the reference's module boundaries (`re
 Numerics: fp32 master weights and fp32 residual stream; bf16 MFMA operands with fp32 accumulation; bf16
 saved activations.  There is no eager fallback: CPU tensors raise.
 """
+import math
 import os
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 
@@ -51,6 +53,13 @@ class _WeightCache:
         val = make(w.detach())
         self._c[key] = (tag, val, weakref.ref(w, lambda _r, k=key, c=self._c: c.pop(k, None) if (k in c and c[k][2]() is None) else None))
         return val
+
+    def current(self, w, kind):
+        """The cached copy of `w` if `get` would return it without making a new one, else None."""
+        hit = self._c.get((id(w), kind))
+        if hit is None or hit[2]() is not w or hit[0] != (w._version, w.data_ptr(), tuple(w.shape), self.epoch):
+            return None
+        return hit[1]
 
     def peek(self, w, kind):
         """The cached copy of `w` if it is current, else None (never creates one)."""
@@ -813,3 +822,184 @@ class FusedLoss(torch.autograd.Function):
             return grad.view(ctx.shape), None, None, None, None
         d = K.scale_by_scalar(grad, gout.contiguous().float(), ctx.weight)
         return d.view(ctx.shape), None, None, None, None
+
+
+# --------------------------------------------------------------------------------------------
+# Operators of encoders that normalise by the root mean square, rotate queries and keys by position and serve in 8 bits.
+class _RMSNorm(torch.autograd.Function):
+    """y = w * h * rstd, h = x + residual.  Saves h as it is stored (in the residual's type) and the fp32 rstd of the unrounded sum."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, out_dtype):
+        grad = any(ctx.needs_input_grad)
+        y, h, rstd = K.rms_norm_fwd(x, weight, residual, eps, out_dtype, want_rstd=grad)
+        ctx.set_materialize_grads(False)
+        ctx.types = (x.dtype, None if residual is None else residual.dtype)
+        if grad:
+            ctx.save_for_backward(x if h is None else h, rstd, weight)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, rstd, weight = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        xt, rt = ctx.types
+        if dy is None:      # only h was used
+            return (dh.to(xt) if need_x and dh is not None else None, torch.zeros_like(weight) if need_w else None,
+                    dh if need_r else None, None, None)
+        other = need_x and rt is not None and rt != xt      # a bf16 branch on an fp32 stream
+        dx, dx2, dw = K.rms_norm_bwd(dy.contiguous(), h, rstd, weight, None if dh is None else dh.contiguous(), want_dw=need_w,
+                                     bf16_copy=other)
+        return (dx2 if other else dx) if need_x else None, dw, dx if need_r else None, None, None
+
+
+def _flat(t, D):
+    """[..., D] as rows, without a copy where the strides allow it."""
+    return t if t.dim() == 2 and t.stride(1) == 1 else t.reshape(-1, D) if t.shape[-1] == D and t.stride(-1) == 1 else \
+        t.contiguous().view(-1, D)
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, out_dtype=None):
+    """Root-mean-square norm of x[..., D] (fp32 or bf16), with the residual's addition where one is given:
+    y = weight * h / sqrt(mean(h^2) + eps), h = x + residual.  Returns y, or (y, h) with a residual: h, in the residual's type, is
+    the residual of the next layer.  The residual is fp32 or of x's type; weight fp32 [D]; y in out_dtype (default bf16, what the
+    products consume).  Differentiable in x, weight and residual.  Sums are fp32 (|h| below 1e18), D <= 16384."""
+    out_dtype = BF16 if out_dtype is None else out_dtype
+    D = x.shape[-1]
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"rms_norm: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
+    if residual is None:
+        return _RMSNorm.apply(_flat(x, D), weight, None, eps, out_dtype).view(x.shape)
+    y, h = _RMSNorm.apply(_flat(x, D), weight, _flat(residual, D), eps, out_dtype)
+    return y.view(x.shape), h.view(x.shape)
+
+
+def _no_grad_only(what, *ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"get_model_amd: {what} is an inference operator without a gradient; call it under torch.no_grad()")
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
+    """rms_norm for 8-bit inference: (q, scale), or (q, scale, h) with a residual.  q e4m3 [M, Kp] and scale e8m0 [M, Kp/128], with
+    M = all leading dimensions and Kp = D rounded up to whole blocks of 128 columns (zeros behind D), are what linear_fp8 takes;
+    value = q * scale.  scale is the smallest power of two that brings the block into e4m3's range: y / scale is then exact, so q
+    carries one rounding.  h keeps x's shape."""
+    _no_grad_only("rms_norm_fp8", x, weight, residual)
+    D = x.shape[-1]
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"rms_norm_fp8: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
+    q, s, h = K.rms_norm_fp8(_flat(x, D), weight, None if residual is None else _flat(residual, D), eps)
+    return (q, s) if h is None else (q, s, h.view(x.shape))
+
+
+def w_fp8(w):
+    """The (q, scale) pair of a weight [N, K], kept like the bf16 copies and made anew when the parameter changes.  A copy made
+    inside a graph capture belongs to that graph and is not kept."""
+    def make(t):
+        q, s = K.quant_blocks_fp8(t)
+        stream = torch.cuda.current_stream(t.device)
+        return q, s, stream, stream.record_event()
+
+    if torch.cuda.is_current_stream_capturing():
+        hit = WEIGHTS.current(w, "fp8")
+        return K.quant_blocks_fp8(w.detach()) if hit is None else hit[:2]
+    q, s, stream, made = WEIGHTS.get(w, "fp8", make)
+    here = torch.cuda.current_stream(w.device)
+    if here != stream:      # made on another stream: wait for it, and keep the memory until this one is done
+        here.wait_event(made)
+        q.record_stream(here)
+        s.record_stream(here)
+    return q, s
+
+
+def linear_fp8(x, weight, bias=None):
+    """x @ weight^T + bias in 8-bit floating point (e4m3, one power-of-two scale per 128 columns of a row of x and per 128 x 128
+    block of the weight), fp32 accumulation, bf16 out.  Inference only.
+
+    x: [..., K] fp32 / bf16, quantised here, or the (q, scale) pair of rms_norm_fp8 / kernels.quant_rows_fp8 (result [M, N]).
+    weight: [N, K] fp32 / bf16 (a Parameter's 8-bit copy is kept, see w_fp8), or the pair of kernels.quant_blocks_fp8.
+    bias: fp32 [N]."""
+    pair = isinstance(x, (tuple, list))
+    wpair = isinstance(weight, (tuple, list))
+    _no_grad_only("linear_fp8", None if pair else x, None if wpair else weight, bias)
+    if not pair and not wpair and x.shape[-1] != weight.shape[-1]:
+        raise ValueError(f"linear_fp8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    if not pair:
+        _need_gpu(x)
+    qw, sw = weight if wpair else w_fp8(weight)
+    if pair:
+        return K.gemm_fp8(x[0], x[1], qw, sw, bias)
+    qx, sx = K.quant_rows_fp8(_flat(x, x.shape[-1]))
+    return K.gemm_fp8(qx, sx, qw, sw, bias).view(*x.shape[:-1], qw.shape[0])
+
+
+def rotary_frequencies(columns, base=10000.0, scaling=None, factor=1.0, original_length=None, beta_fast=32.0, beta_slow=1.0, device=None):
+    """(inv_freq float64 [columns/2], magnitude) of rotary positions over `columns` rotated columns of a head:
+    inv_freq[i] = base^(-2i/columns), stretched `factor`-fold for contexts longer than the trained `original_length`:
+
+      None      as it is                          "linear"  every frequency divided by factor (positions interpolated)
+      "ntk"     base * factor^(c/(c-2)): the lowest frequency divided by factor, the highest kept
+      "yarn"    frequencies that turn more than beta_fast times over original_length are kept, those that turn less than beta_slow
+                times are divided by factor, a linear ramp over the pair index between; magnitude = 0.1 ln(factor) + 1"""
+    if columns <= 0 or columns % 2:
+        raise ValueError(f"rotary_frequencies: an even number of columns is wanted, got {columns}")
+    if not (base > 0 and factor >= 1.0):
+        raise ValueError(f"rotary_frequencies: base {base} has to be positive and factor {factor} at least 1")
+    i = torch.arange(0, columns, 2, dtype=torch.float64)
+    magnitude = 1.0
+    if scaling == "ntk":
+        base = base * factor ** (columns / (columns - 2)) if columns > 2 else base
+    inv = base ** (-i / columns)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if not original_length or not beta_fast > beta_slow > 0 or base <= 1:
+            raise ValueError("rotary_frequencies: 'yarn' needs original_length, beta_fast > beta_slow > 0 and base > 1")
+
+        def pair(turns):      # pair index whose wavelength fits `turns` times into the original length
+            return columns * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), columns - 1)
+        ramp = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / factor * ramp
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rotary_frequencies: unknown scaling {scaling!r}")
+    return inv.to(device) if device is not None else inv, magnitude
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, inv_freq, positions, offset, layout, magnitude):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(inv_freq, positions)
+        ctx.rest = (offset, layout, magnitude)
+        q, k = K.rotary(q, k, inv_freq, positions, offset, layout, magnitude)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        inv_freq, positions = ctx.saved_tensors
+        dq, dk = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
+        if dq is None:
+            out = (None, None if dk is None else K.rotary(dk, None, inv_freq, positions, *ctx.rest, backward=True)[0])
+        else:
+            out = K.rotary(dq, dk, inv_freq, positions, *ctx.rest, backward=True)
+        return out + (None,) * 5
+
+
+def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0):
+    """Rotary positions on queries [B, T, Hq, D] and keys [B, T, Hk, D] (fp32 or bf16; k may be None), e.g. views into a packed
+    projection: -> new contiguous (q, k), or q alone.  The first R = 2 * len(inv_freq) columns of every head turn, pair (u, v) ->
+    (u cos a - v sin a, v cos a + u sin a) * magnitude with a = position * inv_freq; pairs are (i, i + R/2) ("half") or (2i, 2i + 1)
+    ("interleaved").  positions: int32 / int64 [B, T] or [T] on the GPU, e.g. base pairs (angles are formed in 64 bits); without
+    them token t is at offset + t.  inv_freq (float64, on the GPU) and magnitude: see rotary_frequencies.  Differentiable in q, k."""
+    return _Rotary.apply(q, k, inv_freq, positions, offset, layout, magnitude)
+
+
+def rotary_(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0):
+    """rotary in place, for inference: q and k (or the head range of a packed projection that holds both: k None) are overwritten."""
+    _no_grad_only("rotary_", q, k)
+    q, k = K.rotary(q, k, inv_freq, positions, offset, layout, magnitude, inplace=True)
+    return q if k is None else (q, k)

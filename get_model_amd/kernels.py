@@ -3,6 +3,8 @@
 torch is used only to allocate device buffers and to provide the stream; all arithmetic happens in
 libgetmi355.so.  Every function requires CUDA(HIP) tensors and raises RuntimeError otherwise.
 """
+import ctypes
+
 import torch
 
 from . import lib
@@ -337,3 +339,224 @@ def scale_cast_noalloc(dx, rowscale=None, rows_per_sample=0):
     dbias = torch.empty(D, dtype=F32, device=dx.device)
     lib.call("getmi_scale_cast_noalloc", dx, rowscale, rows_per_sample, dz, dbias, 0, M, D)
     return dz, dbias
+
+
+# ---- root-mean-square norm, 8-bit block-scaled products, rotary positions ---------------------------------------------------
+# These check shapes and types first (ValueError, also for CPU tensors), then that every tensor is on one GPU (RuntimeError),
+# and run on the tensors' own GPU whatever the current one is.
+FP8 = torch.float8_e4m3fn
+SCALE = torch.float8_e8m0fnu        # 2^(byte - 127)
+FP8_BLOCK = 128
+_TYPE = {F32: 0, BF16: 1}
+
+
+def _require(ok, what):
+    if not ok:
+        raise ValueError("getmi355: " + what)
+
+
+def _on_gpu(*ts):
+    """All tensors (None is skipped) on one GPU."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("getmi355 kernels need tensors on the GPU (no CPU fallback exists)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"getmi355: tensors on two GPUs ({dev} and {t.device})")
+    return dev
+
+
+def _rows(t, what):
+    """2-D rows of contiguous columns -> distance of the rows in elements (0 for one row that stands for all)."""
+    _require(t.dim() == 2, f"{what} has to be 2-D (rows of columns), got {tuple(t.shape)}")
+    _require(t.stride(1) == 1 or t.shape[1] <= 1, f"the columns of {what} have to be contiguous")
+    _require(t.shape[0] < 2 ** 31 and t.shape[1] < 2 ** 31, f"{what} is too large")
+    return t.stride(0)
+
+
+def _norm_args(x, weight, residual, eps):
+    ldx = _rows(x, "x")
+    _require(x.dtype in _TYPE, f"x has to be float32 or bfloat16, got {x.dtype}")
+    D = x.shape[1]
+    _require(0 < D <= 16384, f"the norm takes 1 to 16384 columns, got {D}")
+    _require(weight.dtype == F32 and weight.shape == (D,) and weight.is_contiguous(),
+             f"the norm's weight has to be contiguous float32 [{D}], got {weight.dtype} {tuple(weight.shape)}")
+    ldr = 0
+    if residual is not None:
+        _require(residual.shape == x.shape, f"residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
+        _require(residual.dtype in (F32, x.dtype), f"the residual has to be float32 or of x's type, got {residual.dtype}")
+        ldr = _rows(residual, "the residual")
+    _require(eps >= 0, f"eps has to be >= 0, got {eps}")
+    return ldx, ldr, D
+
+
+def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out_dtype=BF16, want_rstd=False):
+    """x fp32 / bf16 [M,D] (rows may lie apart), weight fp32 [D] -> (y, h, rstd).  h = x + residual in the residual's type (None
+    without a residual), y = weight * h / sqrt(mean(h^2) + eps) in out_dtype, rstd fp32 [M] (None unless wanted)."""
+    ldx, ldr, D = _norm_args(x, weight, residual, eps)
+    _require(out_dtype in _TYPE, f"out_dtype has to be float32 or bfloat16, got {out_dtype}")
+    dev = _on_gpu(x, weight, residual)
+    M = x.shape[0]
+    y = torch.empty(M, D, dtype=out_dtype, device=dev)
+    h = None if residual is None else torch.empty(M, D, dtype=residual.dtype, device=dev)
+    rstd = torch.empty(M, dtype=F32, device=dev) if want_rstd else None
+    if M:
+        lib.launch("getmi_rmsnorm_fwd", dev, x.data_ptr(), _TYPE[x.dtype], ldx, None if residual is None else residual.data_ptr(),
+                   0 if residual is None else _TYPE[residual.dtype], ldr, weight.data_ptr(), y.data_ptr(), _TYPE[out_dtype],
+                   None if h is None else h.data_ptr(), None if rstd is None else rstd.data_ptr(), M, D, eps)
+    return y, h, rstd
+
+
+def rms_norm_bwd(dy, h, rstd, weight, dh=None, want_dw=True, bf16_copy=False):
+    """-> (dx, dx2, dw).  dy fp32 / bf16 [M,D], h [M,D] (what was normalised; rows may lie apart), dh of h's type or None.
+    dx in h's type is the gradient of x and of the residual alike; dx2 is dx in bf16 (only with bf16_copy and an fp32 h)."""
+    ldh = _rows(h, "h")
+    M, D = h.shape
+    _require(dy.shape == h.shape and dy.dtype in _TYPE and dy.is_contiguous(), "dy has to be contiguous float32 or bfloat16 of h's shape")
+    _require(h.dtype in _TYPE and 0 < D <= 16384, "h has to be float32 or bfloat16 with 1 to 16384 columns")
+    _require(rstd.shape == (M,) and rstd.dtype == F32 and rstd.is_contiguous(), f"rstd has to be contiguous float32 [{M}]")
+    _require(weight.dtype == F32 and weight.shape == (D,) and weight.is_contiguous(), f"weight has to be contiguous float32 [{D}]")
+    _require(dh is None or (dh.shape == h.shape and dh.dtype == h.dtype and dh.is_contiguous()), "dh has to be contiguous, of h's shape and type")
+    _require(not bf16_copy or h.dtype == F32, "a bf16 copy of dx is made next to an fp32 one only")
+    dev = _on_gpu(dy, h, rstd, weight, dh)
+    dx = torch.empty(M, D, dtype=h.dtype, device=dev)
+    dx2 = torch.empty(M, D, dtype=BF16, device=dev) if bf16_copy else None
+    if M == 0:
+        return dx, dx2, torch.zeros(D, dtype=F32, device=dev) if want_dw else None
+    dw = torch.empty(D, dtype=F32, device=dev) if want_dw else None
+    ws = _ws(lib.query("getmi_rmsnorm_bwd_workspace_bytes", M, D), dev) if want_dw else None
+    lib.launch("getmi_rmsnorm_bwd", dev, dy.data_ptr(), _TYPE[dy.dtype], h.data_ptr(), _TYPE[h.dtype], ldh, rstd.data_ptr(),
+               weight.data_ptr(), None if dh is None else dh.data_ptr(), dx.data_ptr(), None if dx2 is None else dx2.data_ptr(),
+               None if dw is None else dw.data_ptr(), M, D, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    return dx, dx2, dw
+
+
+def _fp8_like(rows, scale_rows, cols, device):
+    """Empty (values [rows, Kp], scales [scale_rows, Kp/128]); rows of scales start on 4-byte words."""
+    kb = -(-cols // FP8_BLOCK)
+    q = torch.empty(rows, kb * FP8_BLOCK, dtype=FP8, device=device)
+    s = torch.empty(scale_rows, (kb + 3) // 4 * 4, dtype=SCALE, device=device)
+    return q, s[:, :kb], kb
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
+    """rms_norm_fwd with y left as e4m3 values and power-of-two scales -> (q [M,Kp], scales [M,Kp/128], h)."""
+    ldx, ldr, D = _norm_args(x, weight, residual, eps)
+    dev = _on_gpu(x, weight, residual)
+    M = x.shape[0]
+    q, s, _ = _fp8_like(M, M, D, dev)
+    h = None if residual is None else torch.empty(M, D, dtype=residual.dtype, device=dev)
+    if M:
+        lib.launch("getmi_rmsnorm_fp8", dev, x.data_ptr(), _TYPE[x.dtype], ldx, None if residual is None else residual.data_ptr(),
+                   0 if residual is None else _TYPE[residual.dtype], ldr, weight.data_ptr(), q.data_ptr(), s.data_ptr(), s.stride(0),
+                   None if h is None else h.data_ptr(), M, D, eps)
+    return q, s, h
+
+
+def quant_rows_fp8(x):
+    """x fp32 / bf16 [M,K] -> (q e4m3 [M,Kp], scales [M,Kp/128]): one power-of-two scale per row and 128 columns."""
+    ldx = _rows(x, "x")
+    M, D = x.shape
+    _require(x.dtype in _TYPE and 0 < D <= 16384, f"quantisation takes float32 or bfloat16 with 1 to 16384 columns, got {x.dtype} [{M}, {D}]")
+    dev = _on_gpu(x)
+    q, s, _ = _fp8_like(M, M, D, dev)
+    if M:
+        lib.launch("getmi_rmsnorm_fp8", dev, x.data_ptr(), _TYPE[x.dtype], ldx, None, 0, 0, None, q.data_ptr(), s.data_ptr(),
+                   s.stride(0), None, M, D, 0.0)
+    return q, s
+
+
+def quant_blocks_fp8(w):
+    """weight fp32 / bf16 [N,K] -> (q e4m3 [N,Kp], scales [ceil(N/128),Kp/128]): one power-of-two scale per 128 x 128 block."""
+    ldw = _rows(w, "the weight")
+    N, Kd = w.shape
+    _require(w.dtype in _TYPE and Kd > 0, f"quantisation takes float32 or bfloat16 [N,K], got {w.dtype} [{N}, {Kd}]")
+    dev = _on_gpu(w)
+    q, s, _ = _fp8_like(N, -(-N // FP8_BLOCK), Kd, dev)
+    if N:
+        lib.launch("getmi_quant_blocks_fp8", dev, w.data_ptr(), _TYPE[w.dtype], ldw, q.data_ptr(), s.data_ptr(), s.stride(0), N, Kd)
+    return q, s
+
+
+def _fp8_operand(q, s, rows, what):
+    _require(q.dtype == FP8 and s.dtype == SCALE, f"{what} has to be (float8_e4m3fn, float8_e8m0fnu), got ({q.dtype}, {s.dtype})")
+    ld = _rows(q, what)
+    kb = q.shape[1] // FP8_BLOCK
+    _require(q.shape[1] == kb * FP8_BLOCK and kb > 0, f"{what} has to be padded to whole blocks of 128 columns, got {q.shape[1]}")
+    _require(ld % 16 == 0 and q.data_ptr() % 16 == 0, f"the rows of {what} have to start on 16 bytes")
+    _require(s.shape == (rows, kb), f"the scales of {what} have to be [{rows}, {kb}], got {tuple(s.shape)}")
+    lds = _rows(s, f"the scales of {what}")
+    if rows == 1:       # a single row's distance means nothing
+        lds = (kb + 3) // 4 * 4
+    _require(lds % 4 == 0 and s.data_ptr() % 4 == 0, f"the scale rows of {what} have to start on 4-byte words")
+    if rows:
+        last = s.storage_offset() + (rows - 1) * lds + (kb + 3) // 4 * 4
+        _require(s.untyped_storage().nbytes() >= last, f"the scale rows of {what} have to reach to whole 4-byte words")
+    return ld, lds
+
+
+def gemm_fp8(a, a_scale, b, b_scale, bias=None):
+    """bf16 [M,N] = a[M,Kp] @ b[N,Kp]^T (+ bias fp32 [N]) with the scales of quant_rows_fp8 (a) and quant_blocks_fp8 (b)."""
+    _require(a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[1], f"operands {tuple(a.shape)} and {tuple(b.shape)} do not match")
+    M, N, Kp = a.shape[0], b.shape[0], a.shape[1]
+    lda, lsa = _fp8_operand(a, a_scale, M, "a")
+    ldb, lsb = _fp8_operand(b, b_scale, -(-N // FP8_BLOCK), "b")
+    _require(bias is None or (bias.dtype == F32 and bias.shape == (N,) and bias.is_contiguous()), f"bias has to be contiguous float32 [{N}]")
+    dev = _on_gpu(a, a_scale, b, b_scale, bias)
+    out = torch.empty(M, N, dtype=BF16, device=dev)
+    if M and N:
+        lib.launch("getmi_gemm_fp8", dev, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
+                   None if bias is None else bias.data_ptr(), out.data_ptr(), M, N, Kp, lda, ldb, N, lsa, lsb)
+    return out
+
+
+def _overlaps(t):
+    """May two elements of t share memory?  (Dimensions in order of stride: each has to step over all the smaller ones.)"""
+    end = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < end:
+            return True
+        end = st * n
+    return False
+
+
+def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0, backward=False, inplace=False):
+    """q [B,T,Hq,D] and k [B,T,Hk,D] (or None), fp32 or bf16, any strides with contiguous columns -> rotated (q, k), new contiguous
+    tensors or, inplace, q and k themselves.  inv_freq: float64 [R/2] on the GPU, R <= D rotated columns; positions: int32 / int64
+    [B,T] or [T] (None: offset, offset + 1, ..); layout "half" or "interleaved"; backward: by the opposite angle."""
+    _require(q.dim() == 4, f"q has to be [B, T, heads, D], got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    _require(q.dtype in _TYPE, f"q has to be float32 or bfloat16, got {q.dtype}")
+    _require(layout in ("half", "interleaved"), f"layout has to be 'half' or 'interleaved', got {layout!r}")
+    _require(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq has to be contiguous float64 [R/2]")
+    R = 2 * inv_freq.shape[0]
+    _require(0 < R <= min(D, 2048), f"{R} rotated columns do not fit heads of {D} (at most 2048)")
+    _require(B * T < 2 ** 31, "more than 2^31 tokens")
+    for t, name in ((q, "q"),) if k is None else ((q, "q"), (k, "k")):
+        _require(t.stride(3) == 1 or D == 1, f"the columns of {name} have to be contiguous")
+        _require(not inplace or not _overlaps(t), f"in place needs a {name} whose elements do not share memory")
+    if k is not None:
+        _require(k.dim() == 4 and k.shape[:2] == (B, T) and k.shape[3] == D and k.dtype == q.dtype,
+                 f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+        _require(Hq + k.shape[2] <= 65536, "more than 65536 heads")
+    pb = pt = 0
+    if positions is not None:
+        _require(positions.dtype in (torch.int64, torch.int32), f"positions have to be int64 or int32, got {positions.dtype}")
+        _require(positions.shape in ((B, T), (T,)), f"positions have to be [{B}, {T}] or [{T}], got {tuple(positions.shape)}")
+        _require(offset == 0, "positions and an offset exclude each other")
+        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    dev = _on_gpu(q, k, inv_freq, positions)
+    qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ko = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
+    if B * T * (Hq + (0 if k is None else k.shape[2])):
+        st = q.stride()[:3] + qo.stride()[:3] + ((0,) * 6 if k is None else k.stride()[:3] + ko.stride()[:3])
+        lib.launch("getmi_rotary", dev, q.data_ptr(), qo.data_ptr(), Hq, None if k is None else k.data_ptr(),
+                   None if k is None else ko.data_ptr(), 0 if k is None else k.shape[2], (ctypes.c_int64 * 12)(*st), _TYPE[q.dtype], B, T, D, R,
+                   inv_freq.data_ptr(), None if positions is None else positions.data_ptr(),
+                   int(positions is not None and positions.dtype == torch.int64), pb, pt, offset, int(layout == "interleaved"),
+                   int(backward), magnitude)
+    return qo, ko

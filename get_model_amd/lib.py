@@ -55,6 +55,13 @@ _SIGNATURES = {
     "getmi_adamw_step": (_i, [_vp, _i, _i, _vp, _i, _vp]),
     "getmi_gemm_wgrad_pair_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "getmi_gemm_wgrad_pair": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _i, _vp, _sz, _vp]),
+    "getmi_rmsnorm_fwd": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _i, _vp, _vp, _i, _i, _f, _vp]),
+    "getmi_rmsnorm_fp8": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp]),
+    "getmi_rmsnorm_bwd_workspace_bytes": (_sz, [_i, _i]),
+    "getmi_rmsnorm_bwd": (_i, [_vp, _i, _vp, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]),
+    "getmi_quant_blocks_fp8": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _i, _vp]),
+    "getmi_gemm_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _i, _vp]),
+    "getmi_rotary": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i64, _i64, _i64, _i, _i, _f, _vp]),
     "getmi_set_cu_limit": (_i, [_i]),
     "getmi_cu_count": (_i, []),
 }
@@ -99,6 +106,20 @@ def call(name, *args):
     lib = load()
     fn = getattr(lib, name)
     rc = fn(*[_ptr(a) for a in args], stream_ptr())
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (code {rc}): {lib.getmi_last_error().decode()}")
+
+
+def launch(name, device, *args):
+    """`call` for tensors that may live on another GPU than the current one: the work goes to `device`'s current stream, with
+    that device current.  Pointers and sizes are passed as plain integers (None = null)."""
+    lib = _lib or load()
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
     if rc != 0:
         raise RuntimeError(f"{name} failed (code {rc}): {lib.getmi_last_error().decode()}")
 

@@ -178,6 +178,47 @@ int getmi_gemm_wgrad_pair(const void* Xa, const void* Ya, int N1a, int N2a, int 
                           const void* Xb, const void* Yb, int N1b, int N2b, int ldxb, int ldyb, float* outb, int accumulate_b,
                           int M, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- root-mean-square norm with the residual's addition, beside LayerNorm.  No counterpart in the reference (its encoder
+ *      normalises with nn.LayerNorm, model/transformer.py:198).  Types: 0 = fp32, 1 = bf16.  D <= 16384. --------------------- */
+/* h = x + residual (residual and h may both be null: h is x); y = w * h * rstd; rstd = 1 / sqrt(mean(h^2) + eps), stored where
+ * rstd is not null.  Rows of x and of the residual are ldx / ldr elements apart (0 is allowed: one row for all), y and h are
+ * contiguous.  The residual and h have one type: fp32, or x's own.  y is formed from the unrounded fp32 sum. */
+int getmi_rmsnorm_fwd(const void* x, int x_type, int64_t ldx, const void* residual, int residual_type, int64_t ldr, const float* w,
+                      void* y, int y_type, void* h, float* rstd, int M, int D, float eps, void* stream);
+/* The same with y left in 8 bits, for getmi_gemm_fp8: q is e4m3 [M, Kp], Kp = D rounded up to whole blocks of 128 columns (zeros
+ * behind D), scales [M, lds] holds one byte e + 127 per block: 2^e is the smallest power of two with max|y| <= 448 * 2^e, and
+ * q = e4m3(y * 2^-e).  An all-zero block has scale 1; a block that holds an infinity or a NaN becomes NaN throughout.
+ * w null (then residual too): x itself is quantised, not normalised. */
+int getmi_rmsnorm_fp8(const void* x, int x_type, int64_t ldx, const void* residual, int residual_type, int64_t ldr, const float* w,
+                      void* q, void* scales, int lds, void* h, int M, int D, float eps, void* stream);
+/* dx = dh + rstd * (w*dy - hhat * mean(w*dy*hhat)), hhat = h * rstd: the gradient of x and of the residual alike.  h, dh (may be
+ * null) and dx have h_type; dx2 (may be null, h fp32 only) receives dx once more in bf16.  dw (may be null) = sum_rows dy * hhat,
+ * fp32, summed in a fixed order. */
+size_t getmi_rmsnorm_bwd_workspace_bytes(int M, int D);
+int getmi_rmsnorm_bwd(const void* dy, int dy_type, const void* h, int h_type, int64_t ldh, const float* rstd, const float* w,
+                      const void* dh, void* dx, void* dx2, float* dw, int M, int D, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ---- products in 8-bit floating point (e4m3) with a power-of-two scale for each block of 128.  No counterpart in the
+ *      reference (fp16 / fp32 autocast).  Inference: there is no backward. -------------------------------------------------- */
+/* weight w[N, K] (rows ldw elements apart) -> q e4m3 [N, Kp] and scales [ceil(N/128), lds], one byte per 128 x 128 block. */
+int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void* scales, int lds, int N, int K, void* stream);
+/* out[M, N] (bf16, rows ldo apart) = sum_b 2^(sa[m,b]-127) 2^(sb[n/128,b]-127) sum_{k in block b} A[m,k] B[n,k]  (+ bias[n], fp32).
+ * A[M, K], B[N, K] e4m3, K % 128 == 0 (pad with zeros), rows on 16 bytes; sa[M, lsa], sb[ceil(N/128), lsb] bytes, rows on 4 bytes
+ * and readable up to whole 4-byte words (ceil(K/512)*4 bytes). */
+int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
+                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream);
+
+/* ---- rotary positions on queries and keys.  No counterpart in the reference (its encoder has no positions). --------------- */
+/* q[B, T, hq, D] -> qo and k[B, T, hk, D] -> ko in one launch (hk may be 0); `strides` is a HOST array of 12 element strides:
+ * batch, token, head of q, qo, k, ko; columns are contiguous.  Pair (u, v) of the first R columns -- (i, i + R/2), or (2i, 2i+1)
+ * where interleaved -- becomes (u cos a - v sin a, v cos a + u sin a) * magnitude with a = position * inv_freq[i], formed in 64
+ * bits; columns R .. D-1 are copied.  backward: -a.  In place (qo == q and ko == k) is allowed.  position = pos[b*pb + t*pt]
+ * (int64 where pos64, else int32; device memory) or, where pos is null, offset + t.  inv_freq: R/2 doubles in device memory. */
+int getmi_rotary(const void* q, void* qo, int hq, const void* k, void* ko, int hk, const int64_t* strides, int type, int B, int T,
+                 int D, int R, const double* inv_freq, const void* pos, int pos64, int64_t pb, int64_t pt, int64_t offset,
+                 int interleaved, int backward, float magnitude, void* stream);
+
 /* ---- sharing the GPU with communication kernels.  No counterpart in the reference (its GEMMs come from vendor
  *      libraries).  The persistent GEMM and the weight-gradient GEMM launch one workgroup per CU, each taking the
  *      whole CU; while RCCL's channel workgroups are resident (gradient all-reduce overlapped with backward) some
