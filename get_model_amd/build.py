@@ -17,6 +17,9 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libgetmi355.so")
 SOURCES = ["error.hip", "gemm.hip", "attention.hip", "norm.hip", "rmsnorm.hip", "gemm_fp8.hip", "rotary.hip", "misc.hip", "optim.hip", "capi.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wno-unused-value", "-ffp-contract=fast"]
+# packed fp32 instructions (v_pk_add_f32 and the like, which -O3 forms from ordinary float code) off: some of their forms have
+# given wrong results on MI355X now and then.  hipcc's host pass warns that it does not know the feature: harmless.
+FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("GETMI_EXTRA_HIPCC_FLAGS", "").split()      # experiments (A/B builds via GETMI_LIB)
 
 
@@ -29,12 +32,12 @@ def _stamp(src):
     return h.hexdigest()
 
 
-def _compile(name):
+def _compile(name, force=False):
     src = os.path.join(CSRC, name)
     obj = os.path.join(OBJ, name.replace(".hip", ".o"))
     stamp_file = obj + ".stamp"
     stamp = _stamp(src)
-    if os.path.exists(obj) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
+    if not force and os.path.exists(obj) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
         return obj, False
     cmd = ["hipcc"] + FLAGS + ["-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -45,10 +48,11 @@ def _compile(name):
     return obj, True
 
 
-def build(verbose=True):
+def build(verbose=True, force=False):
+    """Compile what changed (force: everything) and link.  Returns the library's path."""
     os.makedirs(OBJ, exist_ok=True)
     with ThreadPoolExecutor(max_workers=6) as ex:
-        res = list(ex.map(_compile, SOURCES))
+        res = list(ex.map(lambda name: _compile(name, force), SOURCES))
     objs = [o for o, _ in res]
     if any(changed for _, changed in res) or not os.path.exists(LIB):
         cmd = ["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
