@@ -251,6 +251,7 @@ int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void
 }
 int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
                    int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream) {
+    CuScope scope(false);
     return getmi_gemm_fp8_impl(A, sa, B, sb, bias, out, M, N, K, lda, ldb, ldo, lsa, lsb, ST(stream));
 }
 int getmi_rotary(const void* q, void* qo, int hq, const void* k, void* ko, int hk, const int64_t* strides, int type, int B, int T, int D,

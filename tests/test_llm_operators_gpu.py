@@ -269,7 +269,10 @@ PRODUCT_REL = 2.0 ** -15
 SHAPES = [(1, 1, 1), (1, 17, 128), (1, 768, 768), (1, 2304, 300), (2, 130, 1000), (15, 64, 256), (16, 768, 4096), (17, 129, 640),
           (33, 2304, 768), (64, 1024, 512), (65, 100, 384), (127, 255, 129), (201, 768, 768), (255, 768, 2304), (256, 256, 256),
           (257, 257, 257), (300, 1000, 5000), (1000, 2304, 768), (2049, 513, 128), (4020, 768, 768), (1, 5000, 8192), (7, 8192, 1024),
-          (700, 4096, 1024), (8000, 8, 256), (3, 3, 16384)]
+          (700, 4096, 1024), (8000, 8, 256), (3, 3, 16384),
+          # large tiles: few and many of them per CU, two to twenty blocks deep, ragged rows and columns, rows off 16 bytes
+          (4096, 1024, 256), (2100, 2056, 384), (5000, 2304, 768), (20000, 1024, 256), (20001, 1000, 500), (16500, 2304, 512),
+          (3000, 1501, 640), (9001, 1283, 256), (4100, 1025, 2600), (1111, 5003, 300)]
 
 
 @pytest.mark.parametrize("M,N,Kd", SHAPES)
@@ -283,7 +286,7 @@ def test_gemm_fp8(M, N, Kd, bias):
     within(got, ref, ref.abs() * HALF[BF16] + size * PRODUCT_REL + (0 if b is None else b.abs().double() * U), "product")
 
 
-@pytest.mark.parametrize("M,N,Kd", [(1, 48, 256), (20, 33, 128), (130, 260, 384), (513, 768, 1024), (1025, 300, 640)])
+@pytest.mark.parametrize("M,N,Kd", [(1, 48, 256), (20, 33, 128), (130, 260, 384), (513, 768, 1024), (1025, 300, 640), (4097, 2305, 256), (12345, 1536, 1280)])
 def test_gemm_fp8_of_small_integers(M, N, Kd):
     """Small whole numbers: every product and sum is exact, so a row, column or block out of place shows at once."""
     g = torch.Generator(device="cuda").manual_seed(5)
