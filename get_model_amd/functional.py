@@ -869,15 +869,22 @@ def rms_norm(x, weight, residual=None, eps=1e-6, out_dtype=None):
     D = x.shape[-1]
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rms_norm: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
-    if residual is None:
-        return _RMSNorm.apply(_flat(x, D), weight, None, eps, out_dtype).view(x.shape)
-    y, h = _RMSNorm.apply(_flat(x, D), weight, _flat(residual, D), eps, out_dtype)
-    return y.view(x.shape), h.view(x.shape)
+    x2, r2 = _flat(x, D), None if residual is None else _flat(residual, D)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        out = _RMSNorm.apply(x2, weight, r2, eps, out_dtype)
+        y, h = (out, None) if residual is None else out
+    else:
+        y, h, _ = K.rms_norm_fwd(x2, weight, r2, eps, out_dtype)
+    if x.dim() != 2:
+        y, h = y.view(x.shape), None if h is None else h.view(x.shape)
+    return y if h is None else (y, h)
 
 
 def _no_grad_only(what, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"get_model_amd: {what} is an inference operator without a gradient; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"get_model_amd: {what} is an inference operator without a gradient; call it under torch.no_grad()")
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
@@ -890,23 +897,27 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"rms_norm_fp8: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
     q, s, h = K.rms_norm_fp8(_flat(x, D), weight, None if residual is None else _flat(residual, D), eps)
-    return (q, s) if h is None else (q, s, h.view(x.shape))
+    return (q, s) if h is None else (q, s, h if x.dim() == 2 else h.view(x.shape))
+
+
+def _make_w_fp8(t):
+    q, s = K.quant_blocks_fp8(t)
+    made = torch.cuda.Event()
+    made.record(torch.cuda.current_stream(t.device))
+    return q, s, torch._C._cuda_getCurrentRawStream(t.device.index), made
 
 
 def w_fp8(w):
     """The (q, scale) pair of a weight [N, K], kept like the bf16 copies and made anew when the parameter changes.  A copy made
     inside a graph capture belongs to that graph and is not kept."""
-    def make(t):
-        q, s = K.quant_blocks_fp8(t)
-        stream = torch.cuda.current_stream(t.device)
-        return q, s, stream, stream.record_event()
-
+    _need_gpu(w)
     if torch.cuda.is_current_stream_capturing():
         hit = WEIGHTS.current(w, "fp8")
         return K.quant_blocks_fp8(w.detach()) if hit is None else hit[:2]
-    q, s, stream, made = WEIGHTS.get(w, "fp8", make)
-    here = torch.cuda.current_stream(w.device)
-    if here != stream:      # made on another stream: wait for it, and keep the memory until this one is done
+    q, s, stream, made = WEIGHTS.get(w, "fp8", _make_w_fp8)
+    if torch._C._cuda_getCurrentRawStream(q.device.index) != stream:
+        # made on another stream: wait for it, and keep the memory until this one is done
+        here = torch.cuda.current_stream(q.device)
         here.wait_event(made)
         q.record_stream(here)
         s.record_stream(here)
@@ -920,18 +931,14 @@ def linear_fp8(x, weight, bias=None):
     x: [..., K] fp32 / bf16, quantised here, or the (q, scale) pair of rms_norm_fp8 / kernels.quant_rows_fp8 (result [M, N]).
     weight: [N, K] fp32 / bf16 (a Parameter's 8-bit copy is kept, see w_fp8), or the pair of kernels.quant_blocks_fp8.
     bias: fp32 [N]."""
-    pair = isinstance(x, (tuple, list))
-    wpair = isinstance(weight, (tuple, list))
+    pair, wpair = isinstance(x, (tuple, list)), isinstance(weight, (tuple, list))
     _no_grad_only("linear_fp8", None if pair else x, None if wpair else weight, bias)
     if not pair and not wpair and x.shape[-1] != weight.shape[-1]:
         raise ValueError(f"linear_fp8: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
-    if not pair:
-        _need_gpu(x)
     qw, sw = weight if wpair else w_fp8(weight)
-    if pair:
-        return K.gemm_fp8(x[0], x[1], qw, sw, bias)
-    qx, sx = K.quant_rows_fp8(_flat(x, x.shape[-1]))
-    return K.gemm_fp8(qx, sx, qw, sw, bias).view(*x.shape[:-1], qw.shape[0])
+    qx, sx = x if pair else K.quant_rows_fp8(_flat(x, x.shape[-1]))
+    out = K.gemm_fp8(qx, sx, qw, sw, bias)
+    return out if pair or x.dim() == 2 else out.view(*x.shape[:-1], qw.shape[0])
 
 
 def rotary_frequencies(columns, base=10000.0, scaling=None, factor=1.0, original_length=None, beta_fast=32.0, beta_slow=1.0, device=None):
@@ -995,7 +1002,10 @@ def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.
     (u cos a - v sin a, v cos a + u sin a) * magnitude with a = position * inv_freq; pairs are (i, i + R/2) ("half") or (2i, 2i + 1)
     ("interleaved").  positions: int32 / int64 [B, T] or [T] on the GPU, e.g. base pairs (angles are formed in 64 bits); without
     them token t is at offset + t.  inv_freq (float64, on the GPU) and magnitude: see rotary_frequencies.  Differentiable in q, k."""
-    return _Rotary.apply(q, k, inv_freq, positions, offset, layout, magnitude)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, inv_freq, positions, offset, layout, magnitude)
+    q, k = K.rotary(q, k, inv_freq, positions, offset, layout, magnitude)
+    return q if k is None else (q, k)
 
 
 def rotary_(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0):

@@ -343,54 +343,64 @@ def scale_cast_noalloc(dx, rowscale=None, rows_per_sample=0):
 
 # ---- root-mean-square norm, 8-bit block-scaled products, rotary positions ---------------------------------------------------
 # These check shapes and types first (ValueError, also for CPU tensors), then that every tensor is on one GPU (RuntimeError),
-# and run on the tensors' own GPU whatever the current one is.
+# and run on the tensors' own GPU whatever the current one is.  One token's call is bound by this Python: no message is formatted
+# and no object made before a check fails.
 FP8 = torch.float8_e4m3fn
 SCALE = torch.float8_e8m0fnu        # 2^(byte - 127)
 FP8_BLOCK = 128
 _TYPE = {F32: 0, BF16: 1}
 
 
-def _require(ok, what):
-    if not ok:
-        raise ValueError("getmi355: " + what)
+def _refuse(what):
+    raise ValueError("getmi355: " + what)
 
 
 def _on_gpu(*ts):
-    """All tensors (None is skipped) on one GPU."""
+    """The one GPU of all tensors (None is skipped)."""
     dev = None
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("getmi355 kernels need tensors on the GPU (no CPU fallback exists)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"getmi355: tensors on two GPUs ({dev} and {t.device})")
+        if t is not None:
+            d = t.device
+            if d.type != "cuda":
+                raise RuntimeError("getmi355 kernels need tensors on the GPU (no CPU fallback exists)")
+            if dev is None:
+                dev = d
+            elif d != dev:
+                raise RuntimeError(f"getmi355: tensors on two GPUs ({dev} and {d})")
     return dev
 
 
 def _rows(t, what):
     """2-D rows of contiguous columns -> distance of the rows in elements (0 for one row that stands for all)."""
-    _require(t.dim() == 2, f"{what} has to be 2-D (rows of columns), got {tuple(t.shape)}")
-    _require(t.stride(1) == 1 or t.shape[1] <= 1, f"the columns of {what} have to be contiguous")
-    _require(t.shape[0] < 2 ** 31 and t.shape[1] < 2 ** 31, f"{what} is too large")
-    return t.stride(0)
+    if t.dim() != 2:
+        _refuse(f"{what} has to be 2-D (rows of columns), got {tuple(t.shape)}")
+    M, D = t.shape
+    ld, step = t.stride()
+    if step != 1 and D > 1:
+        _refuse(f"the columns of {what} have to be contiguous")
+    if M >= 2 ** 31 or D >= 2 ** 31:
+        _refuse(f"{what} is too large: {M} x {D}")
+    return ld
 
 
 def _norm_args(x, weight, residual, eps):
     ldx = _rows(x, "x")
-    _require(x.dtype in _TYPE, f"x has to be float32 or bfloat16, got {x.dtype}")
+    if x.dtype not in _TYPE:
+        _refuse(f"x has to be float32 or bfloat16, got {x.dtype}")
     D = x.shape[1]
-    _require(0 < D <= 16384, f"the norm takes 1 to 16384 columns, got {D}")
-    _require(weight.dtype == F32 and weight.shape == (D,) and weight.is_contiguous(),
-             f"the norm's weight has to be contiguous float32 [{D}], got {weight.dtype} {tuple(weight.shape)}")
+    if not 0 < D <= 16384:
+        _refuse(f"the norm takes 1 to 16384 columns, got {D}")
+    if weight.dtype != F32 or weight.shape != (D,) or not weight.is_contiguous():
+        _refuse(f"the norm's weight has to be contiguous float32 [{D}], got {weight.dtype} {tuple(weight.shape)}")
     ldr = 0
     if residual is not None:
-        _require(residual.shape == x.shape, f"residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
-        _require(residual.dtype in (F32, x.dtype), f"the residual has to be float32 or of x's type, got {residual.dtype}")
+        if residual.shape != x.shape:
+            _refuse(f"residual {tuple(residual.shape)} and x {tuple(x.shape)} differ in shape")
+        if residual.dtype != F32 and residual.dtype != x.dtype:
+            _refuse(f"the residual has to be float32 or of x's type, got {residual.dtype}")
         ldr = _rows(residual, "the residual")
-    _require(eps >= 0, f"eps has to be >= 0, got {eps}")
+    if not eps >= 0:
+        _refuse(f"eps has to be >= 0, got {eps}")
     return ldx, ldr, D
 
 
@@ -398,7 +408,8 @@ def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out_dtype=BF16, want_rstd=F
     """x fp32 / bf16 [M,D] (rows may lie apart), weight fp32 [D] -> (y, h, rstd).  h = x + residual in the residual's type (None
     without a residual), y = weight * h / sqrt(mean(h^2) + eps) in out_dtype, rstd fp32 [M] (None unless wanted)."""
     ldx, ldr, D = _norm_args(x, weight, residual, eps)
-    _require(out_dtype in _TYPE, f"out_dtype has to be float32 or bfloat16, got {out_dtype}")
+    if out_dtype not in _TYPE:
+        _refuse(f"out_dtype has to be float32 or bfloat16, got {out_dtype}")
     dev = _on_gpu(x, weight, residual)
     M = x.shape[0]
     y = torch.empty(M, D, dtype=out_dtype, device=dev)
@@ -416,12 +427,18 @@ def rms_norm_bwd(dy, h, rstd, weight, dh=None, want_dw=True, bf16_copy=False):
     dx in h's type is the gradient of x and of the residual alike; dx2 is dx in bf16 (only with bf16_copy and an fp32 h)."""
     ldh = _rows(h, "h")
     M, D = h.shape
-    _require(dy.shape == h.shape and dy.dtype in _TYPE and dy.is_contiguous(), "dy has to be contiguous float32 or bfloat16 of h's shape")
-    _require(h.dtype in _TYPE and 0 < D <= 16384, "h has to be float32 or bfloat16 with 1 to 16384 columns")
-    _require(rstd.shape == (M,) and rstd.dtype == F32 and rstd.is_contiguous(), f"rstd has to be contiguous float32 [{M}]")
-    _require(weight.dtype == F32 and weight.shape == (D,) and weight.is_contiguous(), f"weight has to be contiguous float32 [{D}]")
-    _require(dh is None or (dh.shape == h.shape and dh.dtype == h.dtype and dh.is_contiguous()), "dh has to be contiguous, of h's shape and type")
-    _require(not bf16_copy or h.dtype == F32, "a bf16 copy of dx is made next to an fp32 one only")
+    if dy.shape != h.shape or dy.dtype not in _TYPE or not dy.is_contiguous():
+        _refuse("dy has to be contiguous float32 or bfloat16 of h's shape")
+    if h.dtype not in _TYPE or not 0 < D <= 16384:
+        _refuse("h has to be float32 or bfloat16 with 1 to 16384 columns")
+    if rstd.shape != (M,) or rstd.dtype != F32 or not rstd.is_contiguous():
+        _refuse(f"rstd has to be contiguous float32 [{M}]")
+    if weight.dtype != F32 or weight.shape != (D,) or not weight.is_contiguous():
+        _refuse(f"weight has to be contiguous float32 [{D}]")
+    if dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype or not dh.is_contiguous()):
+        _refuse("dh has to be contiguous, of h's shape and type")
+    if bf16_copy and h.dtype != F32:
+        _refuse("a bf16 copy of dx is made next to an fp32 one only")
     dev = _on_gpu(dy, h, rstd, weight, dh)
     dx = torch.empty(M, D, dtype=h.dtype, device=dev)
     dx2 = torch.empty(M, D, dtype=BF16, device=dev) if bf16_copy else None
@@ -436,11 +453,11 @@ def rms_norm_bwd(dy, h, rstd, weight, dh=None, want_dw=True, bf16_copy=False):
 
 
 def _fp8_like(rows, scale_rows, cols, device):
-    """Empty (values [rows, Kp], scales [scale_rows, Kp/128]); rows of scales start on 4-byte words."""
+    """Empty values [rows, Kp] and scales [scale_rows, Kp/128] whose rows start on 4-byte words, and the words' bytes a row."""
     kb = -(-cols // FP8_BLOCK)
-    q = torch.empty(rows, kb * FP8_BLOCK, dtype=FP8, device=device)
-    s = torch.empty(scale_rows, (kb + 3) // 4 * 4, dtype=SCALE, device=device)
-    return q, s[:, :kb], kb
+    pitch = (kb + 3) // 4 * 4
+    return (torch.empty(rows, kb * FP8_BLOCK, dtype=FP8, device=device),
+            torch.empty_strided((scale_rows, kb), (pitch, 1), dtype=SCALE, device=device), pitch)
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
@@ -448,11 +465,11 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     ldx, ldr, D = _norm_args(x, weight, residual, eps)
     dev = _on_gpu(x, weight, residual)
     M = x.shape[0]
-    q, s, _ = _fp8_like(M, M, D, dev)
+    q, s, pitch = _fp8_like(M, M, D, dev)
     h = None if residual is None else torch.empty(M, D, dtype=residual.dtype, device=dev)
     if M:
         lib.launch("getmi_rmsnorm_fp8", dev, x.data_ptr(), _TYPE[x.dtype], ldx, None if residual is None else residual.data_ptr(),
-                   0 if residual is None else _TYPE[residual.dtype], ldr, weight.data_ptr(), q.data_ptr(), s.data_ptr(), s.stride(0),
+                   0 if residual is None else _TYPE[residual.dtype], ldr, weight.data_ptr(), q.data_ptr(), s.data_ptr(), pitch,
                    None if h is None else h.data_ptr(), M, D, eps)
     return q, s, h
 
@@ -461,12 +478,13 @@ def quant_rows_fp8(x):
     """x fp32 / bf16 [M,K] -> (q e4m3 [M,Kp], scales [M,Kp/128]): one power-of-two scale per row and 128 columns."""
     ldx = _rows(x, "x")
     M, D = x.shape
-    _require(x.dtype in _TYPE and 0 < D <= 16384, f"quantisation takes float32 or bfloat16 with 1 to 16384 columns, got {x.dtype} [{M}, {D}]")
+    if x.dtype not in _TYPE or not 0 < D <= 16384:
+        _refuse(f"quantisation takes float32 or bfloat16 with 1 to 16384 columns, got {x.dtype} [{M}, {D}]")
     dev = _on_gpu(x)
-    q, s, _ = _fp8_like(M, M, D, dev)
+    q, s, pitch = _fp8_like(M, M, D, dev)
     if M:
         lib.launch("getmi_rmsnorm_fp8", dev, x.data_ptr(), _TYPE[x.dtype], ldx, None, 0, 0, None, q.data_ptr(), s.data_ptr(),
-                   s.stride(0), None, M, D, 0.0)
+                   pitch, None, M, D, 0.0)
     return q, s
 
 
@@ -474,38 +492,46 @@ def quant_blocks_fp8(w):
     """weight fp32 / bf16 [N,K] -> (q e4m3 [N,Kp], scales [ceil(N/128),Kp/128]): one power-of-two scale per 128 x 128 block."""
     ldw = _rows(w, "the weight")
     N, Kd = w.shape
-    _require(w.dtype in _TYPE and Kd > 0, f"quantisation takes float32 or bfloat16 [N,K], got {w.dtype} [{N}, {Kd}]")
+    if w.dtype not in _TYPE or Kd == 0:
+        _refuse(f"quantisation takes float32 or bfloat16 [N,K], got {w.dtype} [{N}, {Kd}]")
     dev = _on_gpu(w)
-    q, s, _ = _fp8_like(N, -(-N // FP8_BLOCK), Kd, dev)
+    q, s, pitch = _fp8_like(N, -(-N // FP8_BLOCK), Kd, dev)
     if N:
-        lib.launch("getmi_quant_blocks_fp8", dev, w.data_ptr(), _TYPE[w.dtype], ldw, q.data_ptr(), s.data_ptr(), s.stride(0), N, Kd)
+        lib.launch("getmi_quant_blocks_fp8", dev, w.data_ptr(), _TYPE[w.dtype], ldw, q.data_ptr(), s.data_ptr(), pitch, N, Kd)
     return q, s
 
 
 def _fp8_operand(q, s, rows, what):
-    _require(q.dtype == FP8 and s.dtype == SCALE, f"{what} has to be (float8_e4m3fn, float8_e8m0fnu), got ({q.dtype}, {s.dtype})")
+    """Checks of one operand -> distances of its rows of values and of scales in bytes."""
+    if q.dtype != FP8 or s.dtype != SCALE:
+        _refuse(f"{what} has to be (float8_e4m3fn, float8_e8m0fnu), got ({q.dtype}, {s.dtype})")
     ld = _rows(q, what)
-    kb = q.shape[1] // FP8_BLOCK
-    _require(q.shape[1] == kb * FP8_BLOCK and kb > 0, f"{what} has to be padded to whole blocks of 128 columns, got {q.shape[1]}")
-    _require(ld % 16 == 0 and q.data_ptr() % 16 == 0, f"the rows of {what} have to start on 16 bytes")
-    _require(s.shape == (rows, kb), f"the scales of {what} have to be [{rows}, {kb}], got {tuple(s.shape)}")
-    lds = _rows(s, f"the scales of {what}")
-    if rows == 1:       # a single row's distance means nothing
-        lds = (kb + 3) // 4 * 4
-    _require(lds % 4 == 0 and s.data_ptr() % 4 == 0, f"the scale rows of {what} have to start on 4-byte words")
-    if rows:
-        last = s.storage_offset() + (rows - 1) * lds + (kb + 3) // 4 * 4
-        _require(s.untyped_storage().nbytes() >= last, f"the scale rows of {what} have to reach to whole 4-byte words")
+    cols = q.shape[1]
+    kb = cols // FP8_BLOCK
+    if cols % FP8_BLOCK or kb == 0:
+        _refuse(f"{what} has to be padded to whole blocks of 128 columns, got {cols}")
+    if ld % 16 or q.data_ptr() % 16:
+        _refuse(f"the rows of {what} have to start on 16 bytes")
+    if s.shape != (rows, kb):
+        _refuse(f"the scales of {what} have to be [{rows}, {kb}], got {tuple(s.shape)}")
+    lds = _rows(s, "the scales")
+    if rows <= 1:       # a single row's distance means nothing
+        lds = 0
+    if lds % 4 or s.data_ptr() % 4:
+        _refuse(f"the scale rows of {what} have to start on 4-byte words")
     return ld, lds
 
 
 def gemm_fp8(a, a_scale, b, b_scale, bias=None):
     """bf16 [M,N] = a[M,Kp] @ b[N,Kp]^T (+ bias fp32 [N]) with the scales of quant_rows_fp8 (a) and quant_blocks_fp8 (b)."""
-    _require(a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[1], f"operands {tuple(a.shape)} and {tuple(b.shape)} do not match")
-    M, N, Kp = a.shape[0], b.shape[0], a.shape[1]
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        _refuse(f"operands {tuple(a.shape)} and {tuple(b.shape)} do not match")
+    M, Kp = a.shape
+    N = b.shape[0]
     lda, lsa = _fp8_operand(a, a_scale, M, "a")
     ldb, lsb = _fp8_operand(b, b_scale, -(-N // FP8_BLOCK), "b")
-    _require(bias is None or (bias.dtype == F32 and bias.shape == (N,) and bias.is_contiguous()), f"bias has to be contiguous float32 [{N}]")
+    if bias is not None and (bias.dtype != F32 or bias.shape != (N,) or not bias.is_contiguous()):
+        _refuse(f"bias has to be contiguous float32 [{N}]")
     dev = _on_gpu(a, a_scale, b, b_scale, bias)
     out = torch.empty(M, N, dtype=BF16, device=dev)
     if M and N:
@@ -524,39 +550,65 @@ def _overlaps(t):
     return False
 
 
+_Strides = ctypes.c_int64 * 12
+
+
 def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0, backward=False, inplace=False):
     """q [B,T,Hq,D] and k [B,T,Hk,D] (or None), fp32 or bf16, any strides with contiguous columns -> rotated (q, k), new contiguous
     tensors or, inplace, q and k themselves.  inv_freq: float64 [R/2] on the GPU, R <= D rotated columns; positions: int32 / int64
     [B,T] or [T] (None: offset, offset + 1, ..); layout "half" or "interleaved"; backward: by the opposite angle."""
-    _require(q.dim() == 4, f"q has to be [B, T, heads, D], got {tuple(q.shape)}")
+    if q.dim() != 4:
+        _refuse(f"q has to be [B, T, heads, D], got {tuple(q.shape)}")
     B, T, Hq, D = q.shape
-    _require(q.dtype in _TYPE, f"q has to be float32 or bfloat16, got {q.dtype}")
-    _require(layout in ("half", "interleaved"), f"layout has to be 'half' or 'interleaved', got {layout!r}")
-    _require(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq has to be contiguous float64 [R/2]")
+    qb, qt, qh, step = q.stride()
+    dtype = q.dtype
+    if dtype not in _TYPE:
+        _refuse(f"q has to be float32 or bfloat16, got {dtype}")
+    if layout != "half" and layout != "interleaved":
+        _refuse(f"layout has to be 'half' or 'interleaved', got {layout!r}")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        _refuse("inv_freq has to be contiguous float64 [R/2]")
     R = 2 * inv_freq.shape[0]
-    _require(0 < R <= min(D, 2048), f"{R} rotated columns do not fit heads of {D} (at most 2048)")
-    _require(B * T < 2 ** 31, "more than 2^31 tokens")
-    for t, name in ((q, "q"),) if k is None else ((q, "q"), (k, "k")):
-        _require(t.stride(3) == 1 or D == 1, f"the columns of {name} have to be contiguous")
-        _require(not inplace or not _overlaps(t), f"in place needs a {name} whose elements do not share memory")
+    if not 0 < R <= min(D, 2048):
+        _refuse(f"{R} rotated columns do not fit heads of {D} (at most 2048)")
+    if step != 1 and D > 1:
+        _refuse("the columns of q have to be contiguous")
+    Hk = kb = kt = kh = 0
     if k is not None:
-        _require(k.dim() == 4 and k.shape[:2] == (B, T) and k.shape[3] == D and k.dtype == q.dtype,
-                 f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
-        _require(Hq + k.shape[2] <= 65536, "more than 65536 heads")
-    pb = pt = 0
+        if k.dim() != 4 or k.dtype != dtype or k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
+            _refuse(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {dtype}")
+        Hk = k.shape[2]
+        kb, kt, kh, step = k.stride()
+        if step != 1 and D > 1:
+            _refuse("the columns of k have to be contiguous")
+    if B * T >= 2 ** 31 or Hq + Hk > 65536:
+        _refuse(f"at most 2^31 tokens and 65536 heads, got {B * T} and {Hq + Hk}")
+    pb = pt = wide = 0
     if positions is not None:
-        _require(positions.dtype in (torch.int64, torch.int32), f"positions have to be int64 or int32, got {positions.dtype}")
-        _require(positions.shape in ((B, T), (T,)), f"positions have to be [{B}, {T}] or [{T}], got {tuple(positions.shape)}")
-        _require(offset == 0, "positions and an offset exclude each other")
-        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    dev = _on_gpu(q, k, inv_freq, positions)
-    qo = q if inplace else torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ko = k if inplace or k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
-    if B * T * (Hq + (0 if k is None else k.shape[2])):
-        st = q.stride()[:3] + qo.stride()[:3] + ((0,) * 6 if k is None else k.stride()[:3] + ko.stride()[:3])
+        if positions.dtype != torch.int64 and positions.dtype != torch.int32:
+            _refuse(f"positions have to be int64 or int32, got {positions.dtype}")
+        if offset != 0:
+            _refuse("positions and an offset exclude each other")
+        wide = int(positions.dtype == torch.int64)
+        if positions.shape == (B, T):
+            pb, pt = positions.stride()
+        elif positions.shape == (T,):
+            pt = positions.stride(0)
+        else:
+            _refuse(f"positions have to be [{B}, {T}] or [{T}], got {tuple(positions.shape)}")
+    if inplace:
+        if _overlaps(q) or (k is not None and _overlaps(k)):
+            _refuse("in place needs tensors whose elements do not share memory")
+        dev = _on_gpu(q, k, inv_freq, positions)
+        qo, ko = q, k
+        strides = _Strides(qb, qt, qh, qb, qt, qh, kb, kt, kh, kb, kt, kh)
+    else:
+        dev = _on_gpu(q, k, inv_freq, positions)
+        qo = torch.empty(B, T, Hq, D, dtype=dtype, device=dev)
+        ko = None if k is None else torch.empty(B, T, Hk, D, dtype=dtype, device=dev)
+        strides = _Strides(qb, qt, qh, T * Hq * D, Hq * D, D, kb, kt, kh, T * Hk * D, Hk * D, D)
+    if B * T * (Hq + Hk):
         lib.launch("getmi_rotary", dev, q.data_ptr(), qo.data_ptr(), Hq, None if k is None else k.data_ptr(),
-                   None if k is None else ko.data_ptr(), 0 if k is None else k.shape[2], (ctypes.c_int64 * 12)(*st), _TYPE[q.dtype], B, T, D, R,
-                   inv_freq.data_ptr(), None if positions is None else positions.data_ptr(),
-                   int(positions is not None and positions.dtype == torch.int64), pb, pt, offset, int(layout == "interleaved"),
-                   int(backward), magnitude)
+                   None if k is None else ko.data_ptr(), Hk, strides, _TYPE[dtype], B, T, D, R, inv_freq.data_ptr(),
+                   None if positions is None else positions.data_ptr(), wide, pb, pt, offset, layout == "interleaved", backward, magnitude)
     return qo, ko

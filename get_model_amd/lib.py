@@ -113,15 +113,16 @@ def call(name, *args):
 def launch(name, device, *args):
     """`call` for tensors that may live on another GPU than the current one: the work goes to `device`'s current stream, with
     that device current.  Pointers and sizes are passed as plain integers (None = null)."""
-    lib = _lib or load()
+    fn = getattr(_lib or load(), name)
     index = device.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(index)      # torch.cuda.current_stream(device) without the object: 0.1 instead of 2.6 us
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
     if rc != 0:
-        raise RuntimeError(f"{name} failed (code {rc}): {lib.getmi_last_error().decode()}")
+        raise RuntimeError(f"{name} failed (code {rc}): {_lib.getmi_last_error().decode()}")
 
 
 def query(name, *args):

@@ -205,7 +205,7 @@ int getmi_rmsnorm_bwd(const void* dy, int dy_type, const void* h, int h_type, in
 int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void* scales, int lds, int N, int K, void* stream);
 /* out[M, N] (bf16, rows ldo apart) = sum_b 2^(sa[m,b]-127) 2^(sb[n/128,b]-127) sum_{k in block b} A[m,k] B[n,k]  (+ bias[n], fp32).
  * A[M, K], B[N, K] e4m3, K % 128 == 0 (pad with zeros), rows on 16 bytes; sa[M, lsa], sb[ceil(N/128), lsb] bytes, rows on 4 bytes
- * and readable up to whole 4-byte words (ceil(K/512)*4 bytes). */
+ * (read as the whole 4-byte words that hold a row's K/128 bytes). */
 int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
                    int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream);
 

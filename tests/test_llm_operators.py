@@ -61,8 +61,8 @@ def scales(rows, kb, pitch=None):
     lambda: K.gemm_fp8(fp8(4, 128), scales(5, 1), fp8(8, 128), scales(1, 1)),
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1), fp8(129, 128), scales(1, 1)),        # two blocks of rows
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1, pitch=1), fp8(8, 128), scales(1, 1)),     # scale rows off 4-byte words
-    lambda: K.gemm_fp8(fp8(4, 128), torch.full((13,), 127, dtype=torch.uint8).view(K.SCALE).as_strided((4, 1), (4, 1)),
-                       fp8(8, 128), scales(1, 1)),                                     # the last word is not whole
+    lambda: K.gemm_fp8(fp8(4, 128), torch.full((32,), 127, dtype=torch.uint8).view(K.SCALE)[1:].as_strided((4, 1), (4, 1), 1),
+                       fp8(8, 128), scales(1, 1)),                                     # ... all of them
     lambda: K.gemm_fp8(fp8(4, 136)[:, :128], scales(4, 1), fp8(8, 128), scales(1, 1)),     # rows off 16 bytes
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1), fp8(8, 128), scales(1, 1), bias=z(7)),
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1), fp8(8, 128), scales(1, 1), bias=z(8, dtype=BF16)),
