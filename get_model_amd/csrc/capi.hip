@@ -71,7 +71,8 @@ int getmi_rmsnorm_bwd_impl(const void*, int, const void*, int, int64_t, const fl
                            int, void*, size_t, hipStream_t);
 int getmi_quant_blocks_fp8_impl(const void*, int, int64_t, void*, void*, int, int, int, hipStream_t);
 int getmi_gemm_fp8_impl(const void*, const void*, const void*, const void*, const float*, void*, int, int, int, int64_t, int64_t, int64_t,
-                        int, int, hipStream_t);
+                        int, int, void*, size_t, hipStream_t);
+size_t getmi_gemm_fp8_workspace_bytes_impl(int M, int N, int K);
 int getmi_rotary_impl(const void*, void*, int, const void*, void*, int, const int64_t*, int, int, int, int, int, const double*, const void*,
                       int, int64_t, int64_t, int64_t, int, int, float, hipStream_t);
 
@@ -250,10 +251,11 @@ int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void
     return getmi_quant_blocks_fp8_impl(w, w_type, ldw, q, scales, lds, N, K, ST(stream));
 }
 int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
-                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream) {
+                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* workspace, size_t workspace_bytes, void* stream) {
     CuScope scope(false);
-    return getmi_gemm_fp8_impl(A, sa, B, sb, bias, out, M, N, K, lda, ldb, ldo, lsa, lsb, ST(stream));
+    return getmi_gemm_fp8_impl(A, sa, B, sb, bias, out, M, N, K, lda, ldb, ldo, lsa, lsb, workspace, workspace_bytes, ST(stream));
 }
+size_t getmi_gemm_fp8_workspace_bytes(int M, int N, int K) { return getmi_gemm_fp8_workspace_bytes_impl(M, N, K); }
 int getmi_rotary(const void* q, void* qo, int hq, const void* k, void* ko, int hk, const int64_t* strides, int type, int B, int T, int D,
                  int R, const double* inv_freq, const void* pos, int pos64, int64_t pb, int64_t pt, int64_t offset, int interleaved,
                  int backward, float magnitude, void* stream) {

@@ -11,46 +11,212 @@ struct Fp8Args {
     size_t lda, ldb, ldo; int lsa, lsb, M, N, K;
 };
 
-__device__ __forceinline__ i32x8 frag_global(const unsigned char* p) {
-    typedef __attribute__((ext_vector_type(4))) int i32x4_t;
-    const i32x4_t a = *reinterpret_cast<const i32x4_t*>(p), b = *reinterpret_cast<const i32x4_t*>(p + 16);
-    return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
 __device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
+__device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
+    return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+// A lane's 32 bytes of one block of its row: 16-byte chunks c and 4 + c (each load of a wave then covers 64 consecutive bytes of
+// 16 rows).  Both operands are read alike, so the order inside the block does not matter.
+__device__ __forceinline__ i32x8 frag_global(const unsigned char* p) {
+    return join8(*reinterpret_cast<const u32x4*>(p), *reinterpret_cast<const u32x4*>(p + 64));
+}
+// four consecutive outputs of row m from column n on; gran: how many columns of a row can be stored at once (see granularity())
+__device__ __forceinline__ void store_out4(const Fp8Args& p, int m, int n, f32x4 v, int gran) {
+    if (m >= p.M || n >= p.N) return;
+    bf16_t* o = p.out + (size_t)m * p.ldo + n;
+    if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += p.bias[min(n + i, p.N - 1)];
+    }
+    if (gran >= 4) {
+        *reinterpret_cast<uint2*>(o) = pack4bf(v[0], v[1], v[2], v[3]);
+    } else if (gran == 2) {
+        *reinterpret_cast<unsigned*>(o) = pack2bf(v[0], v[1]);
+        if (n + 2 < p.N) *reinterpret_cast<unsigned*>(o + 2) = pack2bf(v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) o[i] = f2bf(v[i]);
+    }
+}
 
-// One wave: 16 rows of A x 64 rows of B, operands straight from global memory.  The B rows are the matrix unit's rows and the A
-// rows its columns, so a lane ends up with four consecutive n of one m.
-__global__ __launch_bounds__(256) void gemm_fp8_kernel(Fp8Args p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
-    const int m0 = blockIdx.y * 16, n0 = (blockIdx.x * 4 + wave) * 64;
-    if (n0 >= p.N) return;
-    const int m = min(m0 + r, p.M - 1);
-    const unsigned char* a = p.A + (size_t)m * p.lda + c * 32;
-    const unsigned char* sa = p.sa + (size_t)m * p.lsa;
+// ------------------------------------------------------------------------------------------------
+// Few rows (M <= 16 MT): the weights' bytes are the time.  A workgroup owns 16 NT rows of B over the whole depth; its W waves take
+// every W-th block of 128 each, straight from global memory into the matrix unit (nothing is reused, so LDS would only delay it),
+// and the W partial sums are joined in LDS in a fixed order.  The B rows are the matrix unit's rows and the A rows its columns, so
+// a lane ends up with four consecutive n of one m.
+// ------------------------------------------------------------------------------------------------
+template <int MT, int NT>
+__global__ __launch_bounds__(1024) void gemm_fp8_rows_kernel(Fp8Args p, int gran) {
+    extern __shared__ __attribute__((aligned(16))) f32x4 part[];      // [W][NT * MT][64]
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6, nkb = p.K >> 7;
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+    const unsigned char *a[MT], *b[NT], *sa[MT];
     const unsigned char* sb = p.sb + (size_t)(n0 >> 7) * p.lsb;
-    const unsigned char* b[4];
-    f32x4 acc[4];
+    f32x4 acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        b[t] = p.B + (size_t)min(n0 + t * 16 + r, p.N - 1) * p.ldb + c * 32;
-        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MT; ++j) {
+        const size_t m = min(m0 + j * 16 + r, p.M - 1);
+        a[j] = p.A + m * p.lda + c * 16;
+        sa[j] = p.sa + m * p.lsa;
     }
-    for (int k = 0; k < p.K; k += 128) {
-        const i32x8 fa = frag_global(a + k);
-        const int xa = sa[k >> 7], xb = sb[k >> 7];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = mfma_fp8(frag_global(b[t] + k), fa, acc[t], xb, xa);
+    for (int i = 0; i < NT; ++i) {
+        b[i] = p.B + (size_t)min(n0 + i * 16 + r, p.N - 1) * p.ldb + c * 16;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (m0 + r >= p.M) return;
+    auto step = [&](auto n_, int kb) {      // n blocks W apart, all their loads first
+        constexpr int U = decltype(n_)::value;
+        i32x8 fb[U][NT], fa[U][MT];
+        unsigned xa[U][MT], xb[U];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+        for (int u = 0; u < U; ++u) {
+            const int k = kb + u * W;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = n0 + t * 16 + 4 * c + i;
-            if (n < p.N) p.out[(size_t)(m0 + r) * p.ldo + n] = f2bf(acc[t][i] + (p.bias ? p.bias[n] : 0.f));
+            for (int i = 0; i < NT; ++i) fb[u][i] = frag_global(b[i] + (size_t)k * 128);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                fa[u][j] = frag_global(a[j] + (size_t)k * 128);
+                xa[u][j] = sa[j][k];
+            }
+            xb[u] = *reinterpret_cast<const unsigned*>(sb + (k & ~3)) >> ((k & 3) * 8);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) acc[i][j] = mfma_fp8(fb[u][i], fa[u][j], acc[i][j], (int)xb[u], (int)xa[u][j]);
+    };
+    constexpr int U = MT * NT <= 2 ? 4 : 2;
+    int kb = wave;
+    for (; kb + (U - 1) * W < nkb; kb += U * W) step(std::integral_constant<int, U>{}, kb);
+    for (; kb < nkb; kb += W) step(std::integral_constant<int, 1>{}, kb);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) part[(wave * NT * MT + i * MT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    for (int t = threadIdx.x; t < NT * MT * 64; t += blockDim.x) {
+        f32x4 v = part[t];
+        for (int w = 1; w < W; ++w) v += part[w * NT * MT * 64 + t];
+        const int l = t & 63, i = (t >> 6) / MT, j = (t >> 6) % MT;
+        store_out4(p, m0 + j * 16 + (l & 15), n0 + i * 16 + (l >> 4) * 4, v, gran);
+    }
+}
+
+__device__ __forceinline__ void glds4(const void* gsrc, void* lds_wave_base) {
+    __builtin_amdgcn_global_load_lds(GLB_PTR(gsrc), LDS_PTR(lds_wave_base), 4, 0, 0);
+}
+template <int N> __device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N > 63 ? 63 : N) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------
+// Products too small to fill the chip with 256 x 256 tiles: BM x BN tiles, 4 waves (2 x 2), a ring of three K-tiles of one block
+// (128 bytes a row, the image of the large kernel), two of them in flight, one barrier per K-tile, several workgroups per CU.
+// The scale words (rows of A, then the tile's one block of B) ride in a 1-KiB slot beside each K-tile.
+// ------------------------------------------------------------------------------------------------
+// wait until at most n K-tiles (OPS operations each) are in flight, n <= MAX
+template <int OPS, int MAX> __device__ __forceinline__ void wait_tiles(int n) {
+    if constexpr (MAX == 0) wait_vm<0>();
+    else if (n >= MAX) wait_vm<MAX * OPS>();
+    else wait_tiles<OPS, MAX - 1>(n);
+}
+
+template <int BM, int BN, int S>
+__global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws) {
+    constexpr int STAGE = (BM + BN) * 128 + 1024, OPS = (BM + BN) / 32 + 1, MT = BM / 32, NT = BN / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1, nkb = p.K >> 7;
+    const int tiles_n = (p.N + BN - 1) / BN, bid = xcd_remap(blockIdx.x, gridDim.x), lid = bid / splits, sp = bid - lid * splits;
+    const int tm = lid / tiles_n, tn = lid - tm * tiles_n;
+    const int kb0 = (int)((int64_t)nkb * sp / splits), nk = (int)((int64_t)nkb * (sp + 1) / splits) - kb0;      // >= 1: splits <= nkb
+    const int m0 = tm * BM, n0 = tn * BN;
+    // 16-byte pieces: wave w's i-th instruction moves rows 8 (4 i + w) .. + 7 of the [A; B] image
+    const unsigned char* src[OPS - 1];
+#pragma unroll
+    for (int i = 0; i < OPS - 1; ++i) {
+        const int row = (i * 4 + wave) * 8 + (lane >> 3), chunk = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
+        src[i] = (row < BM ? p.A + (size_t)min(m0 + row, p.M - 1) * p.lda : p.B + (size_t)min(n0 + row - BM, p.N - 1) * p.ldb) + chunk;
+    }
+    const unsigned char* ssrc = tid < BM ? p.sa + (size_t)min(m0 + tid, p.M - 1) * p.lsa : p.sb + (size_t)(n0 >> 7) * p.lsb;
+    auto issue = [&](int k, int slot) {
+        char* b = smem + slot * STAGE;
+#pragma unroll
+        for (int i = 0; i < OPS - 1; ++i) glds16(src[i] + (size_t)(kb0 + k) * 128, b + (i * 4 + wave) * 1024);
+        glds4(ssrc + ((kb0 + k) & ~3), b + (BM + BN) * 128 + wave * 256);
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int fsw = (r >> 1) & 7;
+    const unsigned lds0 = lds_addr(smem), off0 = r * 128 + ((c ^ fsw) << 4), off1 = r * 128 + (((4 + c) ^ fsw) << 4);
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k)
+        if (k < nk) issue(k, k);
+    int slot = 0;
+    for (int k = 0; k < nk; ++k) {
+        wait_tiles<OPS, S - 2>(nk - 1 - k);      // K-tile k has landed (this wave's share); the S - 2 after it stay in flight
+        phase_barrier();                          // ... every wave's share; and K-tile k - 1 has been read by all
+        if (k + S - 1 < nk) issue(k + S - 1, slot == 0 ? S - 1 : slot - 1);
+        const unsigned b = lds0 + slot * STAGE, ab = b + wm * (BM / 2) * 128, bb = b + (BM + wn * (BN / 2)) * 128, sc = b + (BM + BN) * 128;
+        u32x4 fa[MT][2], fb[NT][2];
+        unsigned sa[MT], sb;
+        // (inline asm: hipcc would wait for every LDS-DMA in flight before a read it can see)
+        asm volatile("ds_read_b32 %0, %1" : "=&v"(sb) : "v"(sc + (BM < 256 ? BM * 4 : 0)) : "memory");
+#pragma unroll
+        for (int i = 0; i < MT; ++i) asm volatile("ds_read_b32 %0, %1 offset:%2" : "=&v"(sa[i]) : "v"(sc + (wm * (BM / 2) + r) * 4), "n"(i * 64) : "memory");
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fa[i][0]) : "v"(ab + off0), "n"(i * 2048) : "memory");
+            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fa[i][1]) : "v"(ab + off1), "n"(i * 2048) : "memory");
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fb[j][0]) : "v"(bb + off0), "n"(j * 2048) : "memory");
+            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fb[j][1]) : "v"(bb + off1), "n"(j * 2048) : "memory");
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(sb) : : "memory");
+#pragma unroll
+        for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(sa[i]), "+v"(fa[i][0]), "+v"(fa[i][1]));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(fb[j][0]), "+v"(fb[j][1]));
+        const int sh = ((kb0 + k) & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                acc[i][j] = mfma_fp8(join8(fb[j][0], fb[j][1]), join8(fa[i][0], fa[i][1]), acc[i][j], (int)(sb >> sh), (int)(sa[i] >> sh));
+        slot = slot == S - 1 ? 0 : slot + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int m = m0 + wm * (BM / 2) + i * 16 + r, n = n0 + wn * (BN / 2) + j * 16 + c * 4;
+            if (splits == 1) store_out4(p, m, n, acc[i][j], gran);
+            else if (m < p.M && n < p.N) *reinterpret_cast<f32x4*>(ws + ((size_t)sp * p.M + m) * ((p.N + 3) & ~3) + n) = acc[i][j];
+        }
+}
+
+// the partial sums of a split product, in the splits' order
+__global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Fp8Args p, int gran, int splits, const float* ws) {
+    const int n4 = (p.N + 3) >> 2;
+    const int64_t all = (int64_t)p.M * n4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i / n4), n = (int)(i - (int64_t)m * n4) * 4;
+        f32x4 v = reinterpret_cast<const f32x4*>(ws)[i];
+        for (int s = 1; s < splits; ++s) v += reinterpret_cast<const f32x4*>(ws)[i + s * all];
+        store_out4(p, m, n, v, gran);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -71,13 +237,6 @@ __global__ __launch_bounds__(256) void gemm_fp8_kernel(Fp8Args p) {
 #define F8_STAGE (F8_BIAS + 2048)
 #define F8_LDS (F8_STAGE + 8 * 2048)
 
-__device__ __forceinline__ void glds4(const void* gsrc, void* lds_wave_base) {
-    __builtin_amdgcn_global_load_lds(GLB_PTR(gsrc), LDS_PTR(lds_wave_base), 4, 0, 0);
-}
-
-template <int N> __device__ __forceinline__ void wait_vm() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N > 63 ? 63 : N) : "memory");
-}
 // at most `n` half-tiles (0..5) younger than the needed one, plus EXTRA stores, outstanding.  A0 half-tiles are 3 operations, the
 // others 2; PH = 1, 2, 3: the phase, i.e. which kind follows the needed one (B1, A1, A0).
 template <int PH, int EXTRA> __device__ __forceinline__ void wait_f8(int n) {
@@ -90,16 +249,12 @@ template <int PH, int EXTRA> __device__ __forceinline__ void wait_f8(int n) {
     else wait_vm<EXTRA>();
 }
 
-__device__ __forceinline__ i32x8 join8(u32x4 a, u32x4 b) {
-    return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
-}
-
 // RB: 16-row blocks of each wave's second 64-row half that are real output (4, 3, 2: tiles of 256, 224, 192 rows).
-// ODD: rows of the output that do not start on 16 bytes, or N % 8 != 0: stored value by value.
-template <int RB, bool ODD>
+// GR: columns of an output row stored at once (8 where rows start on 16 bytes and N % 8 == 0; 2; 1).
+template <int RB, int GR>
 __global__ __launch_bounds__(512, 2) void gemm_fp8_256p_kernel(Fp8Args p, int ntiles, int group_n) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int BM = 128 + 32 * RB, HW = BM / 2, E = (ODD ? 16 : 2) * (4 + RB);
+    constexpr int BM = 128 + 32 * RB, HW = BM / 2, E = 16 / GR * (4 + RB);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3;
@@ -331,13 +486,14 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_256p_kernel(Fp8Args p, int nt
             for (int ps = 0; ps < 2; ++ps) {
                 const int m = m0w + a * 16 + ps * 8 + rrow, n = n0w + rch * 8;
                 const unsigned off = (unsigned)(((size_t)m * p.ldo + n) * 2);
-                if constexpr (!ODD) st_b128<true>(d[ps], (m < mend && n < p.N) ? off : OOB_OFF, rs);
+                if constexpr (GR == 8) st_b128<true>(d[ps], (m < mend && n < p.N) ? off : OOB_OFF, rs);
                 else
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < 8; j += GR) {
                         const unsigned o = (m < mend && n + j < p.N) ? off + 2 * j : OOB_OFF;
                         const unsigned v = d[ps][j >> 1];
-                        if (j & 1) asm volatile("buffer_store_short_d16_hi %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(v), "v"(o), "s"(rs) : "memory");
+                        if (GR == 2) asm volatile("buffer_store_dword %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(v), "v"(o), "s"(rs) : "memory");
+                        else if (j & 1) asm volatile("buffer_store_short_d16_hi %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(v), "v"(o), "s"(rs) : "memory");
                         else asm volatile("buffer_store_short %0, %1, %2, 0 offen\n\ts_nop 1" ::"v"(v), "v"(o), "s"(rs) : "memory");
                     }
             }
@@ -389,47 +545,104 @@ static int pick_group(int M, int N, int K, int tile_m, int grid) {
     return best_g;
 }
 
-template <int RB, bool ODD> static int launch_256p(const Fp8Args& p, hipStream_t st) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_fp8_256p_kernel<RB, ODD>),
+template <int RB, int GR> static int launch_256p(const Fp8Args& p, hipStream_t st) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_fp8_256p_kernel<RB, GR>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, F8_LDS);
     (void)attr;
     constexpr int BM = 128 + 32 * RB;
     const int ntiles = ((p.M + BM - 1) / BM) * ((p.N + 255) / 256), cus = getmi_cu_budget(), grid = ntiles < cus ? ntiles : cus;
-    hipLaunchKernelGGL((gemm_fp8_256p_kernel<RB, ODD>), dim3(grid), dim3(512), F8_LDS, st, p, ntiles, pick_group(p.M, p.N, p.K, BM, grid));
+    hipLaunchKernelGGL((gemm_fp8_256p_kernel<RB, GR>), dim3(grid), dim3(512), F8_LDS, st, p, ntiles, pick_group(p.M, p.N, p.K, BM, grid));
     GETMI_CHECK_LAUNCH("gemm_fp8");
     return GETMI_OK;
 }
-template <bool ODD> static int launch_big(const Fp8Args& p, hipStream_t st) {
-    // tile height: rounds of the CUs x the time of a round (256 rows: 1, 224: 0.93, 192: 0.87 -- the bf16 kernel's measure)
+// Relative time of one round of tiles of 256 / 224 / 192 rows on all CUs.
+static double round_time(int rb) { return rb == 4 ? 1.0 : rb == 3 ? 0.93 : 0.87; }
+template <int GR> static int launch_big(const Fp8Args& p, hipStream_t st) {
     const int cus = getmi_cu_budget(), tn = (p.N + 255) / 256;
-    const double t[3] = {0.87, 0.93, 1.0};
     int best = 4;
     double cost = 0;
     for (int rb = 4; rb >= 2; --rb) {
         const int bm = 128 + 32 * rb, tiles = ((p.M + bm - 1) / bm) * tn;
-        const double c = (double)((tiles + cus - 1) / cus) * t[rb - 2];
+        const double c = (double)((tiles + cus - 1) / cus) * round_time(rb);
         if (cost == 0 || c < cost - 1e-9) { cost = c; best = rb; }
     }
-    return best == 4 ? launch_256p<4, ODD>(p, st) : best == 3 ? launch_256p<3, ODD>(p, st) : launch_256p<2, ODD>(p, st);
+    return best == 4 ? launch_256p<4, GR>(p, st) : best == 3 ? launch_256p<3, GR>(p, st) : launch_256p<2, GR>(p, st);
+}
+
+template <int MT, int NT> static int launch_rows(const Fp8Args& p, int gran, hipStream_t st) {
+    const int nkb = p.K / 128, wgs = ((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
+    const int W = nkb >= 32 && wgs <= 256 ? 16 : nkb >= 16 ? 8 : 4;      // 4, 8 and 16 measure alike where either applies
+    hipLaunchKernelGGL((gemm_fp8_rows_kernel<MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * W),
+                       (size_t)W * MT * NT * 1024, st, p, gran);
+    GETMI_CHECK_LAUNCH("gemm_fp8");
+    return GETMI_OK;
+}
+static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStream_t st) {
+    constexpr int S = 3, lds = S * (128 * 128 + 1024);
+    const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
+    hipLaunchKernelGGL((gemm_fp8_tile_kernel<64, 64, S>), dim3((unsigned)(tiles * splits)), dim3(256), lds, st, p, gran, splits, ws);
+    if (splits > 1) {
+        const int64_t blocks = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p, gran, splits,
+                           (const float*)ws);
+    }
+    GETMI_CHECK_LAUNCH("gemm_fp8");
+    return GETMI_OK;
+}
+
+// Which kernel takes a product: by its shape alone.  Both sides measured on MI355X (us, back to back, operands in rotation):
+//   up to 16 rows    rows kernel: 1 x 8192 x 8192 13.6 (4.9 TB/s) against 64-row tiles 22.5; 8 x 768 x 8192 9.0 against 21.7.  Two
+//                    16-row groups of B a workgroup where both sides are wide (16 x 8192 x 8192 20.0 -> 17.2; 1 row: 13.6 -> 16.6)
+//   up to 32, N <= 4096   rows kernel with two row groups: 8 x 768 x 8192 9.8; at N = 8192 64-row tiles in two splits win, 22 -> 15.6
+//   64 x 64 tiles    a K-tile costs a CU 16 KiB of its one path to the caches (1.1 ns x tiles over the chip), a lone workgroup 0.34 us
+//   256 x 256 tiles  1.15 us a K-tile with few CUs busy, 1.85 with all (the same path: 64 KiB), 3.5 for the tile's ends
+//                    4020 x 768 x 768 8.6 against 12.2, 12060 x 768 x 768 18.3 against 13.3, 2000 x 4096 x 4096 76 against 39
+//   depth of 6144 on and few 64-row tiles: the depth is split and joined by a second kernel (64 x 8192 x 8192 23.5 -> 17.1,
+//                    300 x 768 x 8192 22.9 -> 13.1; at 4096 x 4096 the join costs what it saves: 13.1 -> 13.3)
+enum { ROWS11, ROWS12, ROWS21, TILE, BIG };
+struct Plan { int kind, splits; };
+static Plan plan_of(int M, int N, int K) {
+    if (M <= 16) return Plan{M > 8 && N >= 8192 ? ROWS12 : ROWS11, 1};
+    if (M <= 32 && N <= 4096) return Plan{ROWS21, 1};
+    const int nk = K >> 7;
+    const double t64 = (double)((M + 63) / 64) * ((N + 63) / 64), t256 = (double)((M + 255) / 256) * ((N + 255) / 256);
+    const double small = 2.5 + nk * (t64 * 1.1e-3 > 0.34 ? t64 * 1.1e-3 : 0.34);
+    const double rounds = (double)(((int64_t)t256 + 255) / 256);
+    const double large = 2.0 + rounds * (nk * (1.15 + 0.7 * (t256 < 256 ? t256 / 256 : 1.0)) + 3.5);
+    if (nk >= 2 && large < small) return Plan{BIG, 1};
+    return Plan{TILE, nk >= 48 && t64 <= 128 ? (t64 <= 64 ? 4 : 2) : 1};
+}
+size_t getmi_gemm_fp8_workspace_bytes_impl(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const Plan pl = plan_of(M, N, K);
+    return pl.splits == 1 ? 0 : (size_t)pl.splits * M * ((N + 3) & ~3) * sizeof(float);
+}
+static int granularity(const void* out, int N, int64_t ldo) {
+    const uint64_t all = (uintptr_t)out / 2 | (uint64_t)N | (uint64_t)ldo;
+    return all % 8 == 0 && (uintptr_t)out % 16 == 0 ? 8 : all % 4 == 0 && (uintptr_t)out % 8 == 0 ? 4 : all % 2 == 0 && (uintptr_t)out % 4 == 0 ? 2 : 1;
 }
 
 int getmi_gemm_fp8_impl(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
-                        int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, hipStream_t st) {
+                        int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* workspace, size_t workspace_bytes, hipStream_t st) {
     GETMI_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && K % 128 == 0, "gemm_fp8: M=%d N=%d K=%d (K is a multiple of 128: pad with zeros)", M, N, K);
     if (M == 0 || N == 0) return GETMI_OK;
-    GETMI_CHECK_ARG(A && sa && B && sb && out, "gemm_fp8: null pointer");
+    GETMI_CHECK_ARG(A && sa && B && sb && out && (uintptr_t)out % 2 == 0, "gemm_fp8: null or odd pointer");
     GETMI_CHECK_ARG(((uintptr_t)A | (uintptr_t)B | (uint64_t)lda | (uint64_t)ldb) % 16 == 0 && lda >= 0 && ldb >= 0 && ldo >= N,
-                    "gemm_fp8: operand rows have to start on 16 bytes");
+                    "gemm_fp8: operand rows have to start on 16 bytes, output rows must not overlap");
     GETMI_CHECK_ARG(((uintptr_t)sa | (uintptr_t)sb | (unsigned)lsa | (unsigned)lsb) % 4 == 0 && lsa >= 0 && lsb >= 0,
                     "gemm_fp8: scale rows have to start on 4 bytes");
-    GETMI_CHECK_ARG((M + 15) / 16 <= 65535, "gemm_fp8: M=%d too large", M);
+    GETMI_CHECK_ARG((int64_t)((M + 63) / 64) * ((N + 63) / 64) < 0x7fffffff, "gemm_fp8: M=%d N=%d too large", M, N);
     Fp8Args p{(const unsigned char*)A, (const unsigned char*)sa, (const unsigned char*)B, (const unsigned char*)sb, bias, (bf16_t*)out,
               (size_t)lda, (size_t)ldb, (size_t)ldo, lsa, lsb, M, N, K};
+    const int gran = granularity(out, N, ldo);
     const size_t lim = 0xF0000000ull;      // the large kernel addresses each operand with 32 bits
     const bool fits = (size_t)M * lda < lim && (size_t)N * ldb < lim && (size_t)M * ldo * 2 < lim && (size_t)M * lsa < lim && (size_t)N * lsb < lim;
-    if (K >= 256 && M >= 128 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 64 && fits)
-        return (ldo % 8 == 0 && N % 8 == 0 && (uintptr_t)out % 16 == 0) ? launch_big<false>(p, st) : launch_big<true>(p, st);
-    hipLaunchKernelGGL(gemm_fp8_kernel, dim3((N + 255) / 256, (M + 15) / 16), dim3(256), 0, st, p);
-    GETMI_CHECK_LAUNCH("gemm_fp8");
-    return GETMI_OK;
+    const Plan pl = plan_of(M, N, K);
+    GETMI_CHECK_ARG(pl.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= getmi_gemm_fp8_workspace_bytes_impl(M, N, K)),
+                    "gemm_fp8: workspace of getmi_gemm_fp8_workspace_bytes(M, N, K) needed");
+    if (pl.kind == ROWS11) return launch_rows<1, 1>(p, gran, st);
+    if (pl.kind == ROWS12) return launch_rows<1, 2>(p, gran, st);
+    if (pl.kind == ROWS21) return launch_rows<2, 1>(p, gran, st);
+    if (pl.kind == BIG && fits) return gran == 8 ? launch_big<8>(p, st) : gran >= 2 ? launch_big<2>(p, st) : launch_big<1>(p, st);
+    return launch_tile(p, gran, pl.splits, (float*)workspace, st);
 }

@@ -535,8 +535,12 @@ def gemm_fp8(a, a_scale, b, b_scale, bias=None):
     dev = _on_gpu(a, a_scale, b, b_scale, bias)
     out = torch.empty(M, N, dtype=BF16, device=dev)
     if M and N:
+        ws, need = None, lib.query("getmi_gemm_fp8_workspace_bytes", M, N, Kp) if Kp >= 6144 else 0      # a shallower one is never split
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
         lib.launch("getmi_gemm_fp8", dev, a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(),
-                   None if bias is None else bias.data_ptr(), out.data_ptr(), M, N, Kp, lda, ldb, N, lsa, lsb)
+                   None if bias is None else bias.data_ptr(), out.data_ptr(), M, N, Kp, lda, ldb, N, lsa, lsb,
+                   None if ws is None else ws.data_ptr(), need)
     return out
 
 

@@ -207,7 +207,9 @@ int getmi_quant_blocks_fp8(const void* w, int w_type, int64_t ldw, void* q, void
  * A[M, K], B[N, K] e4m3, K % 128 == 0 (pad with zeros), rows on 16 bytes; sa[M, lsa], sb[ceil(N/128), lsb] bytes, rows on 4 bytes
  * (read as the whole 4-byte words that hold a row's K/128 bytes). */
 int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
-                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* stream);
+                   int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* workspace, size_t workspace_bytes, void* stream);
+/* 0 unless the depth is split (few rows, K >= 6144): fp32 partial sums, joined in a fixed order. */
+size_t getmi_gemm_fp8_workspace_bytes(int M, int N, int K);
 
 /* ---- rotary positions on queries and keys.  No counterpart in the reference (its encoder has no positions). --------------- */
 /* q[B, T, hq, D] -> qo and k[B, T, hk, D] -> ko in one launch (hk may be 0); `strides` is a HOST array of 12 element strides:

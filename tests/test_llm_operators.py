@@ -128,10 +128,11 @@ def test_c_entries_check_before_they_launch():
         ("getmi_rmsnorm_bwd", (p, 0, p, 0, 8, p, p, n, p, n, p, 4, 8, n, 0, n)),       # dw without workspace
         ("getmi_rmsnorm_bwd", (p, 0, p, 1, 8, p, p, n, p, p, n, 4, 8, n, 0, n)),       # bf16 copy next to bf16
         ("getmi_quant_blocks_fp8", (p, 0, 8, p, p, 0, 8, 8, n)),
-        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 100, 128, 128, 4, 4, 4, n)),       # depth not whole blocks
-        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 120, 128, 4, 4, 4, n)),       # rows off 16 bytes
-        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 3, 4, 4, n)),       # output rows overlap
-        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 4, 5, 4, n)),       # scale rows off 4 bytes
+        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 100, 128, 128, 4, 4, 4, n, 0, n)),       # depth not whole blocks
+        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 120, 128, 4, 4, 4, n, 0, n)),       # rows off 16 bytes
+        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 3, 4, 4, n, 0, n)),       # output rows overlap
+        ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 4, 5, 4, n, 0, n)),       # scale rows off 4 bytes
+        ("getmi_gemm_fp8", (p, p, p, p, n, p, 64, 64, 8192, 8192, 8192, 64, 64, 64, n, 0, n)),     # split depth without workspace
         ("getmi_rotary", (p, p, 1, n, n, 0, n, 0, 1, 1, 8, 8, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),      # no strides
         ("getmi_rotary", (p, p, 1, n, n, 0, p, 0, 1, 1, 8, 7, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),      # odd columns
         ("getmi_rotary", (p, p, 1, n, n, 0, p, 0, 1, 1, 8, 16, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),     # more than the head has
@@ -141,7 +142,7 @@ def test_c_entries_check_before_they_launch():
         assert h.getmi_last_error()
     # nothing to do is no error
     assert h.getmi_rmsnorm_fwd(n, 0, 8, n, 0, 0, n, n, 0, n, n, 0, 8, 1e-6, n) == 0
-    assert h.getmi_gemm_fp8(n, n, n, n, n, n, 0, 4, 128, 128, 128, 4, 4, 4, n) == 0
+    assert h.getmi_gemm_fp8(n, n, n, n, n, n, 0, 4, 128, 128, 128, 4, 4, 4, n, 0, n) == 0
     assert h.getmi_rotary(n, n, 0, n, n, 0, n, 0, 1, 1, 8, 8, n, n, 0, 0, 0, 0, 0, 0, 1.0, n) == 0
 
 

@@ -272,7 +272,11 @@ SHAPES = [(1, 1, 1), (1, 17, 128), (1, 768, 768), (1, 2304, 300), (2, 130, 1000)
           (700, 4096, 1024), (8000, 8, 256), (3, 3, 16384),
           # large tiles: few and many of them per CU, two to twenty blocks deep, ragged rows and columns, rows off 16 bytes
           (4096, 1024, 256), (2100, 2056, 384), (5000, 2304, 768), (20000, 1024, 256), (20001, 1000, 500), (16500, 2304, 512),
-          (3000, 1501, 640), (9001, 1283, 256), (4100, 1025, 2600), (1111, 5003, 300)]
+          (3000, 1501, 640), (9001, 1283, 256), (4100, 1025, 2600), (1111, 5003, 300), (20000, 370, 730),
+          (13000, 1026, 300), (26000, 513, 384),
+          # the depth split in two and in four, and the shapes next to those; two row groups of either operand
+          (64, 300, 8192), (100, 767, 8200), (40, 8192, 6144), (33, 5001, 6272), (64, 2048, 6016), (12, 8200, 1024), (9, 8193, 300),
+          (32, 4096, 700), (20, 33, 9000), (31, 8192, 256)]
 
 
 @pytest.mark.parametrize("M,N,Kd", SHAPES)
