@@ -54,40 +54,47 @@ __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v
 template <int T> struct Elem { typedef float type; };
 template <> struct Elem<BF16> { typedef bf16_t type; };
 
-// four consecutive columns of a row; `vec`: the row starts on 16 (fp32) / 8 (bf16) bytes and n is 0 or >= 4
-template <int T> __device__ __forceinline__ float4 load4(const void* base, size_t off, int n, bool vec) {
-    typedef typename Elem<T>::type E;
-    const E* p = reinterpret_cast<const E*>(base) + off;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (n <= 0) return v;
-    if (vec) {
-        if constexpr (T == F32) return *reinterpret_cast<const float4*>(p);
-        else {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            return make_float4(bf2f(u.x & 0xffff), bf2f(u.x >> 16), bf2f(u.y & 0xffff), bf2f(u.y >> 16));
-        }
+// Four consecutive columns of a row as they lie in memory.  Rows may start on any element (odd widths, views): the access is
+// declared to be aligned to an element only, and the hardware takes a lane's 16 or 8 bytes from there in one instruction.
+template <int T> struct Raw;
+template <> struct Raw<F32> { typedef __attribute__((ext_vector_type(4), aligned(4))) float type; };
+template <> struct Raw<BF16> { typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned short type; };
+
+// n: how many of the four exist (<= 0: none, the result is zero)
+template <int T, bool NT> __device__ __forceinline__ typename Raw<T>::type load_raw(const void* base, size_t off, int n) {
+    typedef typename Raw<T>::type V;
+    const typename Elem<T>::type* p = reinterpret_cast<const typename Elem<T>::type*>(base) + off;
+    V v = {0, 0, 0, 0};
+    if (n >= 4) {
+        if constexpr (NT) v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+        else v = *reinterpret_cast<const V*>(p);
+    } else if (n > 0) {
+        v[0] = p[0];
+        if (n > 1) v[1] = p[1];
+        if (n > 2) v[2] = p[2];
     }
-    auto at = [&](int i) { if constexpr (T == F32) return p[i]; else return bf2f(p[i]); };
-    v.x = at(0);
-    if (n > 1) v.y = at(1);
-    if (n > 2) v.z = at(2);
-    if (n > 3) v.w = at(3);
     return v;
 }
-template <int T> __device__ __forceinline__ void store4(void* base, size_t off, int n, bool vec, float4 v) {
-    typedef typename Elem<T>::type E;
-    E* p = reinterpret_cast<E*>(base) + off;
-    if (n <= 0) return;
-    if (vec) {
-        if constexpr (T == F32) *reinterpret_cast<float4*>(p) = v;
-        else *reinterpret_cast<uint2*>(p) = pack4bf(v.x, v.y, v.z, v.w);
-        return;
+__device__ __forceinline__ float4 widen(Raw<F32>::type v) { return make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ float4 widen(Raw<BF16>::type v) { return make_float4(bf2f(v[0]), bf2f(v[1]), bf2f(v[2]), bf2f(v[3])); }
+template <int T> __device__ __forceinline__ float4 load4(const void* base, size_t off, int n) { return widen(load_raw<T, false>(base, off, n)); }
+
+template <int T> __device__ __forceinline__ void store4(void* base, size_t off, int n, float4 f) {
+    typedef typename Raw<T>::type V;
+    typename Elem<T>::type* p = reinterpret_cast<typename Elem<T>::type*>(base) + off;
+    V v;
+    if constexpr (T == F32) v = V{f.x, f.y, f.z, f.w};
+    else {
+        const uint2 u = pack4bf(f.x, f.y, f.z, f.w);
+        v = V{(unsigned short)u.x, (unsigned short)(u.x >> 16), (unsigned short)u.y, (unsigned short)(u.y >> 16)};
     }
-    auto put = [&](int i, float f) { if constexpr (T == F32) p[i] = f; else p[i] = f2bf(f); };
-    put(0, v.x);
-    if (n > 1) put(1, v.y);
-    if (n > 2) put(2, v.z);
-    if (n > 3) put(3, v.w);
+    if (n >= 4) {
+        *reinterpret_cast<V*>(p) = v;
+    } else if (n > 0) {
+        p[0] = v[0];
+        if (n > 1) p[1] = v[1];
+        if (n > 2) p[2] = v[2];
+    }
 }
 
 // sum over the WPR waves of a row; one LDS slot per wave, `red` is re-used every row (hence the second barrier)
@@ -104,39 +111,53 @@ __device__ __forceinline__ float join_waves(float v, float* red, int wave, int w
 
 struct FwdArgs {
     const void* x; const void* res; const float* w; void* y; void* h; float* rstd; unsigned char* scales;
-    size_t ldx, ldr, ldq; int lds; int M, D, wpr; float eps; int vec, norm;
+    size_t ldx, ldr, ldq; int lds; int M, D, wpr; float eps; int norm;
 };
 
 // XT: type of x; RT: type of the residual and of h (NONE: there is none); YT: type of y (FP8: values and scales)
-template <int XT, int RT, int YT, int NV>
+template <int XT, int RT, int YT, int NV, bool NT>
 __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
     __shared__ float red[16];
+    constexpr int RTT = RT == NONE ? F32 : RT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwaves = blockDim.x >> 6;
-    const int rows = nwaves / p.wpr, part = wave & (p.wpr - 1), sub = wave / p.wpr;
-    const bool vec = p.vec != 0;
+    const int rows = nwaves / p.wpr, part = wave & (p.wpr - 1), sub = wave / p.wpr, stride = gridDim.x * rows;
     int col[NV];
     float4 w[NV];
+    typename Raw<XT>::type nx[NV];
+    typename Raw<RTT>::type nr[NV];
+    auto fetch = [&](int row) {      // the next row is on its way while this one is summed up
+        if (row >= p.M) return;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            nx[v] = load_raw<XT, NT>(p.x, (size_t)row * p.ldx + col[v], p.D - col[v]);
+            if constexpr (RT != NONE) nr[v] = load_raw<RTT, NT>(p.res, (size_t)row * p.ldr + col[v], p.D - col[v]);
+        }
+    };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         col[v] = ((v * p.wpr + part) * 64 + lane) * 4;
-        w[v] = p.norm ? load4<F32>(p.w, col[v], p.D - col[v], vec) : make_float4(1.f, 1.f, 1.f, 1.f);
+        w[v] = p.norm ? load4<F32>(p.w, col[v], p.D - col[v]) : make_float4(1.f, 1.f, 1.f, 1.f);
     }
+    fetch(blockIdx.x * rows + sub);
     // block-uniform trip count: rows past M take part in the barriers and touch no memory
-    for (int base = blockIdx.x * rows; base < p.M; base += gridDim.x * rows) {
+    for (int base = blockIdx.x * rows; base < p.M; base += stride) {
         const int row = base + sub;
         const bool on = row < p.M;
         float4 a[NV];
         float s = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int n = on ? p.D - col[v] : 0;
-            a[v] = load4<XT>(p.x, (size_t)row * p.ldx + col[v], n, vec);
+            a[v] = widen(nx[v]);
             if constexpr (RT != NONE) {
-                const float4 r = load4<RT>(p.res, (size_t)row * p.ldr + col[v], n, vec);
+                const float4 r = widen(nr[v]);
                 a[v].x += r.x; a[v].y += r.y; a[v].z += r.z; a[v].w += r.w;
-                store4<RT>(p.h, (size_t)row * p.D + col[v], n, vec, a[v]);
             }
             s += a[v].x * a[v].x + a[v].y * a[v].y + a[v].z * a[v].z + a[v].w * a[v].w;
+        }
+        if (base + stride < p.M) fetch(row + stride);
+        if constexpr (RT != NONE) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) store4<RTT>(p.h, (size_t)row * p.D + col[v], on ? p.D - col[v] : 0, a[v]);
         }
         float rs = 1.f;
         if (p.norm) {
@@ -146,7 +167,6 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int n = on ? p.D - col[v] : 0;
             const float4 y = make_float4(a[v].x * rs * w[v].x, a[v].y * rs * w[v].y, a[v].z * rs * w[v].z, a[v].w * rs * w[v].w);
             if constexpr (YT == FP8) {
                 const unsigned amax = max32(max(max(abs_bits(y.x), abs_bits(y.y)), max(abs_bits(y.z), abs_bits(y.w))));
@@ -157,7 +177,7 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
                     if ((lane & 31) == 0) p.scales[(size_t)row * p.lds + (col[v] >> 7)] = (unsigned char)byte;
                 }
             } else {
-                store4<YT>(p.y, (size_t)row * p.D + col[v], n, vec, y);
+                store4<YT>(p.y, (size_t)row * p.D + col[v], on ? p.D - col[v] : 0, y);
             }
         }
     }
@@ -165,41 +185,58 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
 
 struct BwdArgs {
     const void* dy; const void* h; const float* rstd; const float* w; const void* dh; void* dx; void* dx2; float* partial;
-    size_t ldh; int M, D, wpr, vec;
+    size_t ldh; int M, D, wpr;
 };
 
 // YT: type of dy; HT: type of h, dh and dx; dx2 (may be null): dx once more in bf16, for a bf16 x added to an fp32 residual
-template <int YT, int HT, int NV>
+template <int YT, int HT, int NV, bool NT>
 __global__ __launch_bounds__(1024) void rms_bwd_kernel(BwdArgs p) {
     extern __shared__ __attribute__((aligned(16))) float lds[];      // 16 join slots, then rows * D column sums where rows > 1
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwaves = blockDim.x >> 6;
-    const int rows = nwaves / p.wpr, part = wave & (p.wpr - 1), sub = wave / p.wpr;
-    const bool vec = p.vec != 0;
+    const int rows = nwaves / p.wpr, part = wave & (p.wpr - 1), sub = wave / p.wpr, stride = gridDim.x * rows;
     int col[NV];
     float4 w[NV], aw[NV];
+    typename Raw<YT>::type ny[NV];
+    typename Raw<HT>::type nh[NV], nd[NV];
+    float nrs = 0.f;
+    auto fetch = [&](int row) {
+        if (row >= p.M) return;
+        nrs = p.rstd[row];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            ny[v] = load_raw<YT, NT>(p.dy, (size_t)row * p.D + col[v], p.D - col[v]);
+            nh[v] = load_raw<HT, NT>(p.h, (size_t)row * p.ldh + col[v], p.D - col[v]);
+            if (p.dh) nd[v] = load_raw<HT, NT>(p.dh, (size_t)row * p.D + col[v], p.D - col[v]);
+        }
+    };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         col[v] = ((v * p.wpr + part) * 64 + lane) * 4;
-        w[v] = load4<F32>(p.w, col[v], p.D - col[v], vec);
+        w[v] = load4<F32>(p.w, col[v], p.D - col[v]);
         aw[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ny[v] = typename Raw<YT>::type{0, 0, 0, 0};
+        nh[v] = nd[v] = typename Raw<HT>::type{0, 0, 0, 0};
     }
-    for (int base = blockIdx.x * rows; base < p.M; base += gridDim.x * rows) {
+    fetch(blockIdx.x * rows + sub);
+    for (int base = blockIdx.x * rows; base < p.M; base += stride) {
         const int row = base + sub;
         const bool on = row < p.M;
-        const float rs = on ? p.rstd[row] : 0.f;
+        const float rs = nrs;
         float4 g[NV], hh[NV], r[NV];
         float c = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int n = on ? p.D - col[v] : 0;
-            g[v] = load4<YT>(p.dy, (size_t)row * p.D + col[v], n, vec);
-            hh[v] = load4<HT>(p.h, (size_t)row * p.ldh + col[v], n, vec);
-            r[v] = p.dh ? load4<HT>(p.dh, (size_t)row * p.D + col[v], n, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+            g[v] = on ? widen(ny[v]) : make_float4(0.f, 0.f, 0.f, 0.f);      // (a row past M adds nothing to the column sums)
+            hh[v] = widen(nh[v]);
+            r[v] = widen(nd[v]);
         }
+        if (base + stride < p.M) fetch(row + stride);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             hh[v].x *= rs; hh[v].y *= rs; hh[v].z *= rs; hh[v].w *= rs;
-            aw[v].x += g[v].x * hh[v].x; aw[v].y += g[v].y * hh[v].y; aw[v].z += g[v].z * hh[v].z; aw[v].w += g[v].w * hh[v].w;
+            if (on) {
+                aw[v].x += g[v].x * hh[v].x; aw[v].y += g[v].y * hh[v].y; aw[v].z += g[v].z * hh[v].z; aw[v].w += g[v].w * hh[v].w;
+            }
             g[v].x *= w[v].x; g[v].y *= w[v].y; g[v].z *= w[v].z; g[v].w *= w[v].w;
             c += g[v].x * hh[v].x + g[v].y * hh[v].y + g[v].z * hh[v].z + g[v].w * hh[v].w;
         }
@@ -209,20 +246,20 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(BwdArgs p) {
             const int n = on ? p.D - col[v] : 0;
             const float4 d = make_float4(r[v].x + rs * (g[v].x - hh[v].x * c), r[v].y + rs * (g[v].y - hh[v].y * c),
                                          r[v].z + rs * (g[v].z - hh[v].z * c), r[v].w + rs * (g[v].w - hh[v].w * c));
-            store4<HT>(p.dx, (size_t)row * p.D + col[v], n, vec, d);
-            if (p.dx2) store4<BF16>(p.dx2, (size_t)row * p.D + col[v], n, vec, d);
+            store4<HT>(p.dx, (size_t)row * p.D + col[v], n, d);
+            if (p.dx2) store4<BF16>(p.dx2, (size_t)row * p.D + col[v], n, d);
         }
     }
     if (!p.partial) return;
     float* out = p.partial + (size_t)blockIdx.x * p.D;
     if (rows == 1) {      // every column belongs to one thread
 #pragma unroll
-        for (int v = 0; v < NV; ++v) store4<F32>(out, col[v], p.D - col[v], vec, aw[v]);
+        for (int v = 0; v < NV; ++v) store4<F32>(out, col[v], p.D - col[v], aw[v]);
         return;
     }
     float* sums = lds + 16;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) store4<F32>(sums, (size_t)sub * p.D + col[v], p.D - col[v], vec, aw[v]);
+    for (int v = 0; v < NV; ++v) store4<F32>(sums, (size_t)sub * p.D + col[v], p.D - col[v], aw[v]);
     __syncthreads();
     for (int i = threadIdx.x; i < p.D; i += blockDim.x) {
         float t = 0.f;
@@ -235,7 +272,7 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(BwdArgs p) {
 // block (the second one comes out of the cache)
 template <int WT>
 __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t ldw, unsigned char* q, size_t ldq, unsigned char* scales,
-                                                           int lds, int N, int K, int vec) {
+                                                           int lds, int N, int K) {
     __shared__ unsigned red[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * 128 + (lane & 31) * 4, n = K - c;
@@ -243,7 +280,7 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t
     const int r1 = min(N, (int)(blockIdx.y + 1) * 128);
     unsigned m = 0;
     for (int r = r0; r < r1; r += 8) {
-        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n, vec != 0);
+        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n);
         m = max(m, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w))));
     }
     m = max32(m);
@@ -254,14 +291,13 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t
     const unsigned byte = scale_byte(m);
     const float inv = inv_scale(byte);
     for (int r = r0; r < r1; r += 8) {
-        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n, vec != 0);
+        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n);
         *reinterpret_cast<unsigned*>(q + (size_t)r * ldq + c) = pack4fp8(v.x, v.y, v.z, v.w, inv, m < 0x7f800000u);
     }
     if (threadIdx.x == 0) scales[(size_t)blockIdx.y * lds + blockIdx.x] = (unsigned char)byte;
 }
 
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
-bool vec_ok(const void* p, int type, size_t ld) { return !p || (ld % 4 == 0 && aligned(p, type == F32 ? 16 : 8)); }
 
 // waves per row and chunks per lane for `cols` columns
 struct Shape { int wpr, nv, threads, rows; };
@@ -269,7 +305,7 @@ Shape shape_of(int cols, int M) {
     const int chunks = (cols + 255) / 256;
     Shape s;
     s.wpr = 1;
-    while ((chunks + s.wpr - 1) / s.wpr > 4) s.wpr *= 2;
+    while (s.wpr < 16 && (chunks + s.wpr - 1) / s.wpr > 3) s.wpr *= 2;      // (four chunks' backward spills: only past 12288 columns)
     if (M <= 512) while (s.wpr < chunks && s.wpr < 16) s.wpr *= 2;
     s.nv = (chunks + s.wpr - 1) / s.wpr;
     s.threads = s.wpr <= 4 ? 256 : s.wpr * 64;
@@ -280,22 +316,32 @@ int grid_of(int M, int rows, int cap) {
     const int g = (int)(((int64_t)M + rows - 1) / rows);
     return g > cap ? cap : g;
 }
+int size_of(int type) { return type == F32 ? 4 : type == BF16 ? 2 : type == FP8 ? 1 : 0; }
+// A call that moves well more than the Infinity Cache holds (256 MiB) reads its inputs past the caches ("nt"): 51456 x 768 in bf16 +
+// fp32 forward 92 -> 72 us, 8-bit 86 -> 69, backward 121 -> 102.  A smaller one may find what the kernel before it wrote: there nt
+// loads cost (51456 x 283 fp32 forward 20 -> 25 and backward 35 -> 42, 6000 x 6000 bf16 backward, 288 MB, 53 -> 59).  A template
+// argument: a branch around the loads costs the small calls what nt loads cost them.
+bool streams(size_t bytes) { return bytes > ((size_t)384 << 20); }
 constexpr int MAX_D = 16384;      // 16 waves x 4 chunks x 256 columns
 
-template <int XT, int RT, int YT> int launch_fwd(FwdArgs& a, const Shape& s, hipStream_t st) {
-    const dim3 grid(grid_of(a.M, s.rows, 2048)), block(s.threads);
+template <int XT, int RT, int YT, bool NT> int launch_fwd(FwdArgs& a, const Shape& s, hipStream_t st) {
+    const dim3 grid(grid_of(a.M, s.rows, 1024)), block(s.threads);
     switch (s.nv) {
-        case 1: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 1>), grid, block, 0, st, a); break;
-        case 2: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 2>), grid, block, 0, st, a); break;
-        case 3: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 3>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 4>), grid, block, 0, st, a); break;
+        case 1: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 1, NT>), grid, block, 0, st, a); break;
+        case 2: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 2, NT>), grid, block, 0, st, a); break;
+        case 3: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 3, NT>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((rms_fwd_kernel<XT, RT, YT, 4, NT>), grid, block, 0, st, a); break;
     }
     GETMI_CHECK_LAUNCH("rmsnorm_fwd");
     return GETMI_OK;
 }
+template <int XT, int RT, int YT> int launch_fwd_nt(FwdArgs& a, const Shape& s, hipStream_t st) {
+    return streams((size_t)a.M * a.D * (size_of(XT) + 2 * size_of(RT) + size_of(YT))) ? launch_fwd<XT, RT, YT, true>(a, s, st)
+                                                                                       : launch_fwd<XT, RT, YT, false>(a, s, st);
+}
 template <int XT, int RT> int launch_fwd_y(FwdArgs& a, int yt, const Shape& s, hipStream_t st) {
-    return yt == F32 ? launch_fwd<XT, RT, F32>(a, s, st) : yt == BF16 ? launch_fwd<XT, RT, BF16>(a, s, st)
-                                                                       : launch_fwd<XT, RT, FP8>(a, s, st);
+    return yt == F32 ? launch_fwd_nt<XT, RT, F32>(a, s, st) : yt == BF16 ? launch_fwd_nt<XT, RT, BF16>(a, s, st)
+                                                                       : launch_fwd_nt<XT, RT, FP8>(a, s, st);
 }
 int fwd(FwdArgs& a, int xt, int rt, int yt, hipStream_t st) {
     const Shape s = shape_of(yt == FP8 ? (int)a.ldq : a.D, a.M);
@@ -323,8 +369,7 @@ int getmi_rmsnorm_fwd_impl(const void* x, int xt, int64_t ldx, const void* res, 
     GETMI_CHECK_ARG(!res || rt == F32 || (rt == BF16 && xt == BF16), "rmsnorm_fwd: the residual is fp32 or of x's type");
     GETMI_CHECK_ARG(ldx >= 0 && (!res || ldr >= 0) && eps >= 0.f, "rmsnorm_fwd: negative stride or eps");
     if (!res) rt = NONE;
-    FwdArgs a{x, res, w, y, h, rstd, nullptr, (size_t)ldx, (size_t)ldr, 0, 0, M, D, 1, eps, 0, 1};
-    a.vec = D % 4 == 0 && vec_ok(x, xt, ldx) && (!res || (vec_ok(res, rt, ldr) && vec_ok(h, rt, D))) && vec_ok(w, F32, 4) && vec_ok(y, yt, D);
+    FwdArgs a{x, res, w, y, h, rstd, nullptr, (size_t)ldx, (size_t)ldr, 0, 0, M, D, 1, eps, 1};
     return fwd(a, xt, rt, yt, st);
 }
 
@@ -340,9 +385,7 @@ int getmi_rmsnorm_fp8_impl(const void* x, int xt, int64_t ldx, const void* res, 
     const int ldq = (D + 127) / 128 * 128;
     GETMI_CHECK_ARG(lds >= ldq / 128 && aligned(q, 4), "rmsnorm_fp8: scale row of %d bytes for %d blocks, or q not on 4 bytes", lds, ldq / 128);
     if (!res) rt = NONE;
-    FwdArgs a{x, res, w, q, h, nullptr, reinterpret_cast<unsigned char*>(scales), (size_t)ldx, (size_t)ldr, (size_t)ldq, lds, M, D, 1, eps, 0,
-              w != nullptr};
-    a.vec = D % 4 == 0 && vec_ok(x, xt, ldx) && (!res || (vec_ok(res, rt, ldr) && vec_ok(h, rt, D))) && vec_ok(w, F32, 4);
+    FwdArgs a{x, res, w, q, h, nullptr, reinterpret_cast<unsigned char*>(scales), (size_t)ldx, (size_t)ldr, (size_t)ldq, lds, M, D, 1, eps, w != nullptr};
     return fwd(a, xt, rt, FP8, st);
 }
 
@@ -352,22 +395,25 @@ int getmi_quant_blocks_fp8_impl(const void* w, int wt, int64_t ldw, void* q, voi
     const int nb = (N + 127) / 128, kb = (K + 127) / 128;
     GETMI_CHECK_ARG(w && q && scales && (wt == F32 || wt == BF16) && ldw >= 0, "quant_blocks_fp8: null pointer, type or stride");
     GETMI_CHECK_ARG(lds >= kb && aligned(q, 4) && nb <= 65535, "quant_blocks_fp8: scale row of %d bytes for %d blocks, q not on 4 bytes or N too large", lds, kb);
-    const int vec = K % 4 == 0 && vec_ok(w, wt, ldw);
-    if (wt == F32) hipLaunchKernelGGL(quant_blocks_kernel<F32>, dim3(kb, nb), dim3(256), 0, st, w, (size_t)ldw, (unsigned char*)q, (size_t)kb * 128, (unsigned char*)scales, lds, N, K, vec);
-    else hipLaunchKernelGGL(quant_blocks_kernel<BF16>, dim3(kb, nb), dim3(256), 0, st, w, (size_t)ldw, (unsigned char*)q, (size_t)kb * 128, (unsigned char*)scales, lds, N, K, vec);
+    if (wt == F32) hipLaunchKernelGGL(quant_blocks_kernel<F32>, dim3(kb, nb), dim3(256), 0, st, w, (size_t)ldw, (unsigned char*)q, (size_t)kb * 128, (unsigned char*)scales, lds, N, K);
+    else hipLaunchKernelGGL(quant_blocks_kernel<BF16>, dim3(kb, nb), dim3(256), 0, st, w, (size_t)ldw, (unsigned char*)q, (size_t)kb * 128, (unsigned char*)scales, lds, N, K);
     GETMI_CHECK_LAUNCH("quant_blocks_fp8");
     return GETMI_OK;
 }
 
 int getmi_colreduce_impl(const float* partial, float* out0, float* out1, float* out2, int R, int C, int accumulate, hipStream_t st);
 
-template <int YT, int HT> static void launch_bwd(const BwdArgs& a, const Shape& s, int grid, size_t lds, hipStream_t st) {
+template <int YT, int HT, bool NT> static void launch_bwd(const BwdArgs& a, const Shape& s, int grid, size_t lds, hipStream_t st) {
     switch (s.nv) {
-        case 1: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 1>), dim3(grid), dim3(s.threads), lds, st, a); break;
-        case 2: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 2>), dim3(grid), dim3(s.threads), lds, st, a); break;
-        case 3: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 3>), dim3(grid), dim3(s.threads), lds, st, a); break;
-        default: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 4>), dim3(grid), dim3(s.threads), lds, st, a); break;
+        case 1: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 1, NT>), dim3(grid), dim3(s.threads), lds, st, a); break;
+        case 2: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 2, NT>), dim3(grid), dim3(s.threads), lds, st, a); break;
+        case 3: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 3, NT>), dim3(grid), dim3(s.threads), lds, st, a); break;
+        default: hipLaunchKernelGGL((rms_bwd_kernel<YT, HT, 4, NT>), dim3(grid), dim3(s.threads), lds, st, a); break;
     }
+}
+template <int YT, int HT> static void launch_bwd(const BwdArgs& a, const Shape& s, int grid, size_t lds, bool nt, hipStream_t st) {
+    if (nt) launch_bwd<YT, HT, true>(a, s, grid, lds, st);
+    else launch_bwd<YT, HT, false>(a, s, grid, lds, st);
 }
 
 int getmi_rmsnorm_bwd_impl(const void* dy, int yt, const void* h, int ht, int64_t ldh, const float* rstd, const float* w, const void* dh,
@@ -380,11 +426,11 @@ int getmi_rmsnorm_bwd_impl(const void* dy, int yt, const void* h, int ht, int64_
                     "rmsnorm_bwd: dw needs a workspace of getmi_rmsnorm_bwd_workspace_bytes(M, D)");
     const Shape s = shape_of(D, M);
     const int g = bwd_grid(M, s);
-    BwdArgs a{dy, h, rstd, w, dh, dx, dx2, dw ? reinterpret_cast<float*>(workspace) : nullptr, (size_t)ldh, M, D, s.wpr, 0};
-    a.vec = D % 4 == 0 && vec_ok(dy, yt, D) && vec_ok(h, ht, ldh) && vec_ok(w, F32, 4) && vec_ok(dh, ht, D) && vec_ok(dx, ht, D) && vec_ok(dx2, BF16, D);
-    const size_t lds = (16 + (s.rows > 1 ? (size_t)s.rows * D : 0)) * sizeof(float);      // at most 4 x 1024 or 2 x 2048 columns
-    if (yt == F32) { if (ht == F32) launch_bwd<F32, F32>(a, s, g, lds, st); else launch_bwd<F32, BF16>(a, s, g, lds, st); }
-    else { if (ht == F32) launch_bwd<BF16, F32>(a, s, g, lds, st); else launch_bwd<BF16, BF16>(a, s, g, lds, st); }
+    BwdArgs a{dy, h, rstd, w, dh, dx, dx2, dw ? reinterpret_cast<float*>(workspace) : nullptr, (size_t)ldh, M, D, s.wpr};
+    const bool nt = streams((size_t)M * D * (size_of(yt) + (dh ? 3 : 2) * size_of(ht) + (dx2 ? 2 : 0)));
+    const size_t lds = (16 + (s.rows > 1 ? (size_t)s.rows * D : 0)) * sizeof(float);      // at most 4 x 768 or 2 x 1536 columns
+    if (yt == F32) { if (ht == F32) launch_bwd<F32, F32>(a, s, g, lds, nt, st); else launch_bwd<F32, BF16>(a, s, g, lds, nt, st); }
+    else { if (ht == F32) launch_bwd<BF16, F32>(a, s, g, lds, nt, st); else launch_bwd<BF16, BF16>(a, s, g, lds, nt, st); }
     GETMI_CHECK_LAUNCH("rmsnorm_bwd");
     return dw ? getmi_colreduce_impl(a.partial, dw, nullptr, nullptr, g, D, 0, st) : GETMI_OK;
 }

@@ -44,7 +44,7 @@ __device__ __forceinline__ float2 cos_sin(double pos, double f) {
 
 // V consecutive elements as fp32
 template <int T, int V> struct Pack { float v[V]; };
-template <int T, int V> __device__ __forceinline__ Pack<T, V> load(const void* base, int64_t off) {
+template <int T, int V, bool NT> __device__ __forceinline__ Pack<T, V> load(const void* base, int64_t off) {
     Pack<T, V> r;
     if constexpr (T == F32) {
         const float* p = reinterpret_cast<const float*>(base) + off;
@@ -52,7 +52,7 @@ template <int T, int V> __device__ __forceinline__ Pack<T, V> load(const void* b
         else {
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(p + i);
+                const float4 f = load_f4<NT>(p + i);
                 r.v[i] = f.x; r.v[i + 1] = f.y; r.v[i + 2] = f.z; r.v[i + 3] = f.w;
             }
         }
@@ -60,7 +60,7 @@ template <int T, int V> __device__ __forceinline__ Pack<T, V> load(const void* b
         const bf16_t* p = reinterpret_cast<const bf16_t*>(base) + off;
         if constexpr (V == 1) r.v[0] = bf2f(p[0]);
         else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const uint4 u = load_u4<NT>(p);
             const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) { r.v[2 * i] = bf2f(w[i] & 0xffff); r.v[2 * i + 1] = bf2f(w[i] >> 16); }
@@ -74,24 +74,29 @@ template <int T, int V> __device__ __forceinline__ void store(void* base, int64_
         if constexpr (V == 1) p[0] = r.v[0];
         else {
 #pragma unroll
-            for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
+            for (int i = 0; i < V; i += 4) store_f4<false>(p + i, make_float4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]));
         }
     } else {
         bf16_t* p = reinterpret_cast<bf16_t*>(base) + off;
         if constexpr (V == 1) p[0] = f2bf(r.v[0]);
-        else *reinterpret_cast<uint4*>(p) = make_uint4(pack2bf(r.v[0], r.v[1]), pack2bf(r.v[2], r.v[3]), pack2bf(r.v[4], r.v[5]), pack2bf(r.v[6], r.v[7]));
+        else store_u4<false>(p, make_uint4(pack2bf(r.v[0], r.v[1]), pack2bf(r.v[2], r.v[3]), pack2bf(r.v[4], r.v[5]), pack2bf(r.v[6], r.v[7])));
     }
 }
 
 // V: elements per access (8 bf16 / 4 fp32, or 1 where an address, a stride or a width does not allow 16 bytes).
 // threadIdx.x walks the pieces of one head -- first the rotated ones, then (copy) the ones that pass through -- and
-// threadIdx.y the (token, head) pairs of the workgroup's tokens; blockIdx.y shares the heads of few tokens out.
-template <int T, bool HALF, int V>
+// threadIdx.y the (token, head) pairs of the workgroup's tokens; blockIdx.y shares the heads of few tokens out.  A piece is one
+// access, or two (TWO) where a pair's halves lie apart: at e and e2.  Two pieces are in flight per lane, their loads first:
+// lanes that rotate and lanes that copy load and store together and part only for the arithmetic.
+template <int T, bool HALF, int V, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(Args p) {
-    extern __shared__ __attribute__((aligned(16))) float2 table[];      // [tb][R/2]
-    const int half = p.R >> 1, tok0 = blockIdx.x * p.tb, tid = threadIdx.y * blockDim.x + threadIdx.x;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr bool TWO = HALF || V == 1;
+    const int half = p.R >> 1, tok0 = blockIdx.x * p.tb, tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
     const int tokens = min(p.tb, p.ntok - tok0);
-    for (int i = tid; i < tokens * half; i += blockDim.x * blockDim.y) {
+    int64_t* base = reinterpret_cast<int64_t*>(smem);                      // [tb][4]: where the token starts in q, qo, k, ko
+    float2* table = reinterpret_cast<float2*>(smem + p.tb * 32);           // [tb][R/2]
+    for (int i = tid; i < tokens * half; i += threads) {
         const int tl = i / half, f = i - tl * half, b = (tok0 + tl) / p.T, t = (tok0 + tl) - b * p.T;
         int64_t at = p.offset + t;
         if (p.pos) {
@@ -100,50 +105,77 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args p) {
         }
         const float2 cs = cos_sin((double)at, p.inv_freq[f]);
         table[i] = make_float2(cs.x * p.magnitude, cs.y * p.magnitude * p.sign);
+        if (f == 0) {
+            base[tl * 4 + 0] = b * p.q.ib + t * p.q.it;
+            base[tl * 4 + 1] = b * p.q.ob + t * p.q.ot;
+            base[tl * 4 + 2] = b * p.k.ib + t * p.k.it;
+            base[tl * 4 + 3] = b * p.k.ob + t * p.k.ot;
+        }
     }
     __syncthreads();
-    const int heads = p.q.heads + p.k.heads;
-    const int turned = HALF ? half / V : p.R / V, pieces = turned + (p.copy ? (p.D - p.R) / V : 0);
-    const int step = blockDim.y * gridDim.y;
-    for (int j = blockIdx.y * blockDim.y + threadIdx.y; j < tokens * heads; j += step) {
-        const int tl = j / heads, hh = j - tl * heads, tok = tok0 + tl, b = tok / p.T, t = tok - b * p.T;
-        const bool is_q = hh < p.q.heads;
-        const Side& s = is_q ? p.q : p.k;
-        const int h = is_q ? hh : hh - p.q.heads;
-        const int64_t ib = b * s.ib + t * s.it + h * s.ih, ob = b * s.ob + t * s.ot + h * s.oh;
-        const float2* cs = table + tl * half;
-        for (int c = threadIdx.x; c < pieces; c += blockDim.x) {
-            if (c >= turned) {
-                const int e = p.R + (c - turned) * V;
-                store<T, V>(s.out, ob + e, load<T, V>(s.in, ib + e));
-            } else if constexpr (HALF) {
-                const int e = c * V;
-                Pack<T, V> u = load<T, V>(s.in, ib + e), v = load<T, V>(s.in, ib + half + e);
+    const int heads = p.q.heads + p.k.heads, turned = TWO ? half / V : p.R / V;
+    const int pieces = turned + (p.copy ? (TWO ? (p.D - p.R + 2 * V - 1) / (2 * V) : (p.D - p.R) / V) : 0);
+    const int step = blockDim.y * gridDim.y, dt = step / heads, dh = step - dt * heads;
+    for (int c = threadIdx.x; c < pieces; c += blockDim.x) {
+        const bool turn = c < turned;
+        int e = c * V, e2 = 0;
+        if constexpr (HALF) {
+            e = turn ? c * V : p.R + (c - turned) * 2 * V;
+            e2 = turn ? half + c * V : e + V;
+        } else if constexpr (TWO) {
+            e = 2 * c;
+            e2 = e + 1;
+        }
+        const bool second = TWO && e2 < p.D;
+        int j = blockIdx.y * blockDim.y + threadIdx.y, tl = j / heads, h = j - tl * heads;
+        while (tl < tokens) {
+            int64_t at_out[2];
+            void* out[2];
+            const float2* cs[2];
+            Pack<T, V> u[2], v[2];
+            bool on[2];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float2 w = cs[e + i];
-                    const float a = u.v[i], d = v.v[i];
-                    u.v[i] = a * w.x - d * w.y;
-                    v.v[i] = d * w.x + a * w.y;
+            for (int i = 0; i < 2; ++i) {
+                on[i] = tl < tokens;
+                if (on[i]) {
+                    const bool is_q = h < p.q.heads;
+                    const int hh = is_q ? h : h - p.q.heads;
+                    const void* in = is_q ? p.q.in : p.k.in;
+                    const int64_t at = base[tl * 4 + (is_q ? 0 : 2)] + hh * (is_q ? p.q.ih : p.k.ih);
+                    out[i] = is_q ? p.q.out : p.k.out;
+                    at_out[i] = base[tl * 4 + (is_q ? 1 : 3)] + hh * (is_q ? p.q.oh : p.k.oh);
+                    cs[i] = table + tl * half;
+                    u[i] = load<T, V, NT>(in, at + e);
+                    if (second) v[i] = load<T, V, NT>(in, at + e2);
                 }
-                store<T, V>(s.out, ob + e, u);
-                store<T, V>(s.out, ob + half + e, v);
-            } else if constexpr (V > 1) {
-                const int e = c * V;
-                Pack<T, V> u = load<T, V>(s.in, ib + e);
+                tl += dt;
+                h += dh;
+                if (h >= heads) { h -= heads; ++tl; }
+            }
 #pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float2 w = cs[(e + i) >> 1];
-                    const float a = u.v[i], d = u.v[i + 1];
-                    u.v[i] = a * w.x - d * w.y;
-                    u.v[i + 1] = d * w.x + a * w.y;
+            for (int i = 0; i < 2; ++i) {
+                if (!on[i]) continue;
+                if (turn) {
+                    if constexpr (TWO) {
+#pragma unroll
+                        for (int x = 0; x < V; ++x) {
+                            const float2 w = cs[i][c * V + x];
+                            const float a = u[i].v[x], d = v[i].v[x];
+                            u[i].v[x] = a * w.x - d * w.y;
+                            v[i].v[x] = d * w.x + a * w.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < V; x += 2) {
+                            const float2 w = cs[i][(e + x) >> 1];
+                            const float a = u[i].v[x], d = u[i].v[x + 1];
+                            u[i].v[x] = a * w.x - d * w.y;
+                            u[i].v[x + 1] = d * w.x + a * w.y;
+                        }
+                    }
                 }
-                store<T, V>(s.out, ob + e, u);
-            } else if ((c & 1) == 0) {      // one lane writes both halves of its pair: in place is safe
-                const float2 w = cs[c >> 1];
-                const float a = load<T, 1>(s.in, ib + c).v[0], d = load<T, 1>(s.in, ib + c + 1).v[0];
-                store<T, 1>(s.out, ob + c, Pack<T, 1>{{a * w.x - d * w.y}});
-                store<T, 1>(s.out, ob + c + 1, Pack<T, 1>{{d * w.x + a * w.y}});
+                store<T, V>(out[i], at_out[i] + e, u[i]);
+                if (second) store<T, V>(out[i], at_out[i] + e2, v[i]);
             }
         }
     }
@@ -155,7 +187,8 @@ bool wide(const Side& s, int size) {
 }
 
 template <int T, bool HALF, int V> void launch(Args& a, hipStream_t st) {
-    const int half = a.R / 2, pieces = (HALF ? half : a.R) / V + (a.copy ? (a.D - a.R) / V : 0);
+    constexpr bool TWO = HALF || V == 1;
+    const int half = a.R / 2, pieces = (TWO ? half : a.R) / V + (a.copy ? (TWO ? (a.D - a.R + 2 * V - 1) / (2 * V) : (a.D - a.R) / V) : 0);
     const int bx = pieces < 256 ? pieces : 256, by = 256 / bx, heads = a.q.heads + a.k.heads;
     // tokens per workgroup: enough that its 256 threads form one cosine and sine each, as long as that leaves 4 workgroups a CU
     a.tb = 256 / half < 1 ? 1 : 256 / half;
@@ -163,7 +196,13 @@ template <int T, bool HALF, int V> void launch(Args& a, hipStream_t st) {
     const int blocks = (a.ntok + a.tb - 1) / a.tb, rounds = (a.tb * heads + by - 1) / by;
     int gy = 1;
     while (blocks * gy < 512 && gy * 2 <= rounds && gy < 64) gy *= 2;
-    hipLaunchKernelGGL((rotary_kernel<T, HALF, V>), dim3(blocks, gy), dim3(bx, by), (size_t)a.tb * half * sizeof(float2), st, a);
+    const size_t lds = (size_t)a.tb * (32 + half * sizeof(float2));
+    // More than the Infinity Cache holds (256 MiB), and whole 128-byte lines an access: the inputs are read past the caches ("nt";
+    // 32768 x 18 x 128 fp32 126 -> 115 us, interleaved bf16 58 -> 55).  Halves of 64 bytes share lines and lose: 63 -> 65.
+    const size_t size = T == F32 ? 4 : 2;
+    const bool nt = V > 1 && 2 * size * a.ntok * heads * a.D > ((size_t)256 << 20) && (!HALF || half * size % 128 == 0);
+    if (nt) hipLaunchKernelGGL((rotary_kernel<T, HALF, V, (V > 1)>), dim3(blocks, gy), dim3(bx, by), lds, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, HALF, V, false>), dim3(blocks, gy), dim3(bx, by), lds, st, a);
 }
 
 }  // namespace
@@ -187,6 +226,7 @@ int getmi_rotary_impl(const void* q, void* qo, int hq, const void* k, void* ko, 
     a.copy = R < D && !((hq == 0 || q == qo) && (hk == 0 || k == ko));
     a.magnitude = magnitude; a.sign = backward ? -1.f : 1.f;
     const int size = type == F32 ? 4 : 2, v = 16 / size;
+    // 16 bytes an access: every row, the second half of the rotated columns and the columns behind them start on 16 bytes
     const bool w = wide(a.q, size) && wide(a.k, size) && (interleaved ? R : R / 2) % v == 0 && (!a.copy || (D - R) % v == 0);
     if (type == F32) {
         if (interleaved) { if (w) launch<F32, false, 4>(a, st); else launch<F32, false, 1>(a, st); }
