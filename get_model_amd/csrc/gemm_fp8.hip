@@ -2,6 +2,7 @@
 // with e4m3 operands.  v_mfma_scale_f32_16x16x128_f8f6f4 takes one block of 128 in its depth and applies one power-of-two scale
 // per row and 32 columns by itself, so the scales cost no vector instruction and the accumulators are plain fp32 sums.
 #include "gemm_pipe.h"
+#include <atomic>
 #include <type_traits>
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
@@ -545,10 +546,25 @@ static int pick_group(int M, int N, int K, int tile_m, int grid) {
     return best_g;
 }
 
+// More than 64 KiB of dynamic LDS has to be allowed for, once on every GPU that runs the kernel.
+template <typename F> static int allow_lds(F kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return GETMI_OK;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        getmi_set_error("gemm_fp8: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+        return GETMI_ERR_LAUNCH;
+    }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return GETMI_OK;
+}
+
 template <int RB, int GR> static int launch_256p(const Fp8Args& p, hipStream_t st) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_fp8_256p_kernel<RB, GR>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, F8_LDS);
-    (void)attr;
+    static std::atomic<uint64_t> done{0};
+    if (const int rc = allow_lds(gemm_fp8_256p_kernel<RB, GR>, F8_LDS, done)) return rc;
     constexpr int BM = 128 + 32 * RB;
     const int ntiles = ((p.M + BM - 1) / BM) * ((p.N + 255) / 256), cus = getmi_cu_budget(), grid = ntiles < cus ? ntiles : cus;
     hipLaunchKernelGGL((gemm_fp8_256p_kernel<RB, GR>), dim3(grid), dim3(512), F8_LDS, st, p, ntiles, pick_group(p.M, p.N, p.K, BM, grid));
@@ -613,7 +629,7 @@ static Plan plan_of(int M, int N, int K) {
     return Plan{TILE, nk >= 48 && t64 <= 128 ? (t64 <= 64 ? 4 : 2) : 1};
 }
 size_t getmi_gemm_fp8_workspace_bytes_impl(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fff0000 || N > 0x7fff0000) return 0;
     const Plan pl = plan_of(M, N, K);
     return pl.splits == 1 ? 0 : (size_t)pl.splits * M * ((N + 3) & ~3) * sizeof(float);
 }
@@ -624,7 +640,7 @@ static int granularity(const void* out, int N, int64_t ldo) {
 
 int getmi_gemm_fp8_impl(const void* A, const void* sa, const void* B, const void* sb, const float* bias, void* out, int M, int N, int K,
                         int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* workspace, size_t workspace_bytes, hipStream_t st) {
-    GETMI_CHECK_ARG(M >= 0 && N >= 0 && K > 0 && K % 128 == 0, "gemm_fp8: M=%d N=%d K=%d (K is a multiple of 128: pad with zeros)", M, N, K);
+    GETMI_CHECK_ARG(M >= 0 && N >= 0 && M <= 0x7fff0000 && N <= 0x7fff0000 && K > 0 && K <= 0x7fff0000 && K % 128 == 0, "gemm_fp8: M=%d N=%d K=%d (K is a multiple of 128: pad with zeros)", M, N, K);
     if (M == 0 || N == 0) return GETMI_OK;
     GETMI_CHECK_ARG(A && sa && B && sb && out && (uintptr_t)out % 2 == 0, "gemm_fp8: null or odd pointer");
     GETMI_CHECK_ARG(((uintptr_t)A | (uintptr_t)B | (uint64_t)lda | (uint64_t)ldb) % 16 == 0 && lda >= 0 && ldb >= 0 && ldo >= N,

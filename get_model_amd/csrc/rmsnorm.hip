@@ -136,6 +136,8 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         col[v] = ((v * p.wpr + part) * 64 + lane) * 4;
+        nx[v] = typename Raw<XT>::type{0, 0, 0, 0};
+        nr[v] = typename Raw<RTT>::type{0, 0, 0, 0};
         w[v] = p.norm ? load4<F32>(p.w, col[v], p.D - col[v]) : make_float4(1.f, 1.f, 1.f, 1.f);
     }
     fetch(blockIdx.x * rows + sub);
@@ -323,6 +325,7 @@ int size_of(int type) { return type == F32 ? 4 : type == BF16 ? 2 : type == FP8 
 // argument: a branch around the loads costs the small calls what nt loads cost them.
 bool streams(size_t bytes) { return bytes > ((size_t)384 << 20); }
 constexpr int MAX_D = 16384;      // 16 waves x 4 chunks x 256 columns
+constexpr int MAX_M = 0x7fff0000;      // the row loops step past the end in 32 bits
 
 template <int XT, int RT, int YT, bool NT> int launch_fwd(FwdArgs& a, const Shape& s, hipStream_t st) {
     const dim3 grid(grid_of(a.M, s.rows, 1024)), block(s.threads);
@@ -362,7 +365,7 @@ size_t getmi_rmsnorm_bwd_workspace_bytes_impl(int M, int D) {
 
 int getmi_rmsnorm_fwd_impl(const void* x, int xt, int64_t ldx, const void* res, int rt, int64_t ldr, const float* w, void* y, int yt,
                            void* h, float* rstd, int M, int D, float eps, hipStream_t st) {
-    GETMI_CHECK_ARG(M >= 0 && D > 0 && D <= MAX_D, "rmsnorm_fwd: M=%d D=%d (D <= %d)", M, D, MAX_D);
+    GETMI_CHECK_ARG(M >= 0 && M <= MAX_M && D > 0 && D <= MAX_D, "rmsnorm_fwd: M=%d D=%d (D <= %d)", M, D, MAX_D);
     if (M == 0) return GETMI_OK;
     GETMI_CHECK_ARG(x && w && y && (res == nullptr) == (h == nullptr), "rmsnorm_fwd: null pointer");
     GETMI_CHECK_ARG((xt == F32 || xt == BF16) && (yt == F32 || yt == BF16), "rmsnorm_fwd: types are 0 (fp32) and 1 (bf16)");
@@ -375,7 +378,7 @@ int getmi_rmsnorm_fwd_impl(const void* x, int xt, int64_t ldx, const void* res, 
 
 int getmi_rmsnorm_fp8_impl(const void* x, int xt, int64_t ldx, const void* res, int rt, int64_t ldr, const float* w, void* q,
                            void* scales, int lds, void* h, int M, int D, float eps, hipStream_t st) {
-    GETMI_CHECK_ARG(M >= 0 && D > 0 && D <= MAX_D, "rmsnorm_fp8: M=%d D=%d (D <= %d)", M, D, MAX_D);
+    GETMI_CHECK_ARG(M >= 0 && M <= MAX_M && D > 0 && D <= MAX_D, "rmsnorm_fp8: M=%d D=%d (D <= %d)", M, D, MAX_D);
     if (M == 0) return GETMI_OK;
     GETMI_CHECK_ARG(x && q && scales && (res == nullptr) == (h == nullptr), "rmsnorm_fp8: null pointer");
     GETMI_CHECK_ARG(xt == F32 || xt == BF16, "rmsnorm_fp8: types are 0 (fp32) and 1 (bf16)");
@@ -390,7 +393,7 @@ int getmi_rmsnorm_fp8_impl(const void* x, int xt, int64_t ldx, const void* res, 
 }
 
 int getmi_quant_blocks_fp8_impl(const void* w, int wt, int64_t ldw, void* q, void* scales, int lds, int N, int K, hipStream_t st) {
-    GETMI_CHECK_ARG(N >= 0 && K > 0, "quant_blocks_fp8: N=%d K=%d", N, K);
+    GETMI_CHECK_ARG(N >= 0 && N <= MAX_M && K > 0 && K <= MAX_M, "quant_blocks_fp8: N=%d K=%d", N, K);
     if (N == 0) return GETMI_OK;
     const int nb = (N + 127) / 128, kb = (K + 127) / 128;
     GETMI_CHECK_ARG(w && q && scales && (wt == F32 || wt == BF16) && ldw >= 0, "quant_blocks_fp8: null pointer, type or stride");
@@ -418,7 +421,7 @@ template <int YT, int HT> static void launch_bwd(const BwdArgs& a, const Shape& 
 
 int getmi_rmsnorm_bwd_impl(const void* dy, int yt, const void* h, int ht, int64_t ldh, const float* rstd, const float* w, const void* dh,
                            void* dx, void* dx2, float* dw, int M, int D, void* workspace, size_t workspace_bytes, hipStream_t st) {
-    GETMI_CHECK_ARG(M > 0 && D > 0 && D <= MAX_D, "rmsnorm_bwd: M=%d D=%d (D <= %d)", M, D, MAX_D);
+    GETMI_CHECK_ARG(M > 0 && M <= MAX_M && D > 0 && D <= MAX_D, "rmsnorm_bwd: M=%d D=%d (D <= %d)", M, D, MAX_D);
     GETMI_CHECK_ARG(dy && h && rstd && w && dx && ldh >= 0, "rmsnorm_bwd: null pointer or negative stride");
     GETMI_CHECK_ARG((yt == F32 || yt == BF16) && (ht == F32 || ht == BF16), "rmsnorm_bwd: types are 0 (fp32) and 1 (bf16)");
     GETMI_CHECK_ARG(!dx2 || ht == F32, "rmsnorm_bwd: a second, bf16 dx only next to an fp32 one");

@@ -214,7 +214,7 @@ int getmi_rotary_impl(const void* q, void* qo, int hq, const void* k, void* ko, 
     GETMI_CHECK_ARG(B >= 0 && T >= 0 && hq >= 0 && hk >= 0 && D > 0, "rotary: B=%d T=%d heads=%d,%d D=%d", B, T, hq, hk, D);
     GETMI_CHECK_ARG(R > 0 && R % 2 == 0 && R <= D && R <= 2048, "rotary: %d rotated columns of %d (even, at most 2048)", R, D);
     if (B == 0 || T == 0 || hq + hk == 0) return GETMI_OK;
-    GETMI_CHECK_ARG((int64_t)B * T <= 0x7fffffff && (int64_t)hq + hk <= 65536, "rotary: more than 2^31 tokens or 65536 heads");
+    GETMI_CHECK_ARG((int64_t)B * T <= 0x7fff0000 && (int64_t)hq + hk <= 65536, "rotary: more than 0x7fff0000 tokens or 65536 heads");
     GETMI_CHECK_ARG(strides && inv_freq && (hq == 0 || (q && qo)) && (hk == 0 || (k && ko)), "rotary: null pointer");
     GETMI_CHECK_ARG(type == F32 || type == BF16, "rotary: types are 0 (fp32) and 1 (bf16)");
     Args a{};

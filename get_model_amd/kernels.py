@@ -349,6 +349,7 @@ FP8 = torch.float8_e4m3fn
 SCALE = torch.float8_e8m0fnu        # 2^(byte - 127)
 FP8_BLOCK = 128
 _TYPE = {F32: 0, BF16: 1}
+_MOST = 0x7fff0000                  # rows / tokens: the kernels step past the end in 32 bits
 
 
 def _refuse(what):
@@ -378,7 +379,7 @@ def _rows(t, what):
     ld, step = t.stride()
     if step != 1 and D > 1:
         _refuse(f"the columns of {what} have to be contiguous")
-    if M >= 2 ** 31 or D >= 2 ** 31:
+    if M > _MOST or D > _MOST:
         _refuse(f"{what} is too large: {M} x {D}")
     return ld
 
@@ -554,6 +555,34 @@ def _overlaps(t):
     return False
 
 
+def _share(q, k):
+    """May q[B,T,Hq,D] and k[B,T,Hk,D], neither of which overlaps itself, share elements?  No if their addresses lie apart, or if they
+    are parts of one layout: equal strides, and k's start one more step in the order of the strides."""
+    if not q.numel() or not k.numel():
+        return False
+    span = [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))) for t in (q, k)]
+    if span[0][1] <= span[1][0] or span[1][1] <= span[0][0]:
+        return False
+    low, high = (q, k) if q.data_ptr() <= k.data_ptr() else (k, q)
+    step = (high.data_ptr() - low.data_ptr()) // q.element_size()
+    dims = []
+    for a, b, st, st2 in zip(low.shape, high.shape, low.stride(), high.stride()):
+        if max(a, b) > 1:
+            if a > 1 and b > 1 and st != st2:
+                return True
+            dims.append((st if a > 1 else st2, a, b))
+    ends, placed = [1, 1], False
+    for st, a, b in sorted(dims):
+        if not placed and step < st:
+            if step < ends[0]:
+                return True
+            ends, placed = [step + ends[1]] * 2, True
+        if st < max(ends):
+            return True
+        ends = [st * max(a, b)] * 2 if placed else [st * a, st * b]
+    return not placed and step < ends[0]
+
+
 _Strides = ctypes.c_int64 * 12
 
 
@@ -585,8 +614,10 @@ def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.
         kb, kt, kh, step = k.stride()
         if step != 1 and D > 1:
             _refuse("the columns of k have to be contiguous")
-    if B * T >= 2 ** 31 or Hq + Hk > 65536:
-        _refuse(f"at most 2^31 tokens and 65536 heads, got {B * T} and {Hq + Hk}")
+    if B * T > _MOST or Hq + Hk > 65536:
+        _refuse(f"at most {_MOST} tokens and 65536 heads, got {B * T} and {Hq + Hk}")
+    if not -2 ** 53 < offset < 2 ** 53:
+        _refuse(f"offset {offset} is not below 2^53")
     pb = pt = wide = 0
     if positions is not None:
         if positions.dtype != torch.int64 and positions.dtype != torch.int32:
@@ -601,7 +632,7 @@ def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.
         else:
             _refuse(f"positions have to be [{B}, {T}] or [{T}], got {tuple(positions.shape)}")
     if inplace:
-        if _overlaps(q) or (k is not None and _overlaps(k)):
+        if _overlaps(q) or (k is not None and (_overlaps(k) or _share(q, k))):
             _refuse("in place needs tensors whose elements do not share memory")
         dev = _on_gpu(q, k, inv_freq, positions)
         qo, ko = q, k

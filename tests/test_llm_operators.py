@@ -73,6 +73,7 @@ def test_products_refuse(call):
 
 
 INV = Fn.rotary_frequencies(8)[0]
+X = z(2, 3, 6, 8)
 
 
 @pytest.mark.parametrize("call", [
@@ -90,10 +91,33 @@ INV = Fn.rotary_frequencies(8)[0]
     lambda: K.rotary(z(2, 3, 8, 4).transpose(2, 3), None, INV),                        # columns apart
     lambda: K.rotary(z(2, 3, 1, 8).expand(2, 3, 4, 8), None, INV, inplace=True),       # elements share memory
     lambda: K.rotary(z(1, 1, 1, 4098), None, torch.ones(1025, dtype=F64)),
+    lambda: K.rotary(z(1, 1, 1, 8), None, INV, offset=2 ** 53),
+    lambda: K.rotary(X, X, INV, inplace=True),                                         # q and k the same, shifted, interleaved
+    lambda: K.rotary(X[:, :-1], X[:, 1:], INV, inplace=True),
+    lambda: K.rotary(X[:, :, :4], X[:, :, 3:], INV, inplace=True),
+    lambda: K.rotary(X[..., 0:8], X.view(2, 3, 48)[:, :, 4:44].unflatten(2, (5, 8)), INV, inplace=True),
 ])
 def test_rotary_refuses(call):
     with pytest.raises(ValueError):
         call()
+
+
+@pytest.mark.parametrize("Hq,Hk", [(4, 2), (1, 5), (3, 3), (6, 0)])
+def test_parts_of_one_layout_do_not_share(Hq, Hk):
+    """Queries and keys of a packed projection, in either order, heads before or behind the tokens: exactly the calls that touch no
+    element twice pass (the rule against a count of every element)."""
+    B, T, D = 2, 3, 8
+    H = Hq + Hk + 1
+    for buf in (torch.arange(B * T * H * D).view(B, T, H, D), torch.arange(B * H * T * D).view(B, H, T, D).transpose(1, 2),
+                torch.arange(T * B * H * D).view(T, B, H, D).transpose(0, 1)):
+        for a in range(H - Hq + 1):
+            for b in range(H - Hk + 1):
+                q, k = buf[:, :, a:a + Hq], buf[:, :, b:b + Hk]
+                both = torch.cat((q.reshape(-1), k.reshape(-1)))
+                assert K._share(q, k) == (both.unique().numel() < both.numel()), (a, b)
+    rows = torch.arange(B * (T + 1) * H * D).view(B, T + 1, H, D)
+    if Hk:
+        assert K._share(rows[:, :T, :Hk], rows[:, 1:, :Hk])
 
 
 def test_no_cpu_fallback():

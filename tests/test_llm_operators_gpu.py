@@ -465,6 +465,32 @@ def test_rotary_nothing_to_do_and_masked_values():
     assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], want[~bad])
 
 
+def test_rows_past_four_gigabytes():
+    """Rows so far apart that their distances from the first pass 32 bits, in elements and in bytes."""
+    far = torch.zeros(5 * 2 ** 30, dtype=torch.uint8, device="cuda")
+    qa, qb = operands(16500, 2304, 512)
+    a = far.view(K.FP8).as_strided((16500, 512), (320000, 1))      # large tiles by its shape: more than their 32 bits reach
+    a.copy_(qa[0])
+    assert torch.equal(K.gemm_fp8(a, qa[1], *qb), K.gemm_fp8(*qa, *qb))
+    qa, qb = operands(3, 40, 256)
+    a = far.view(K.FP8).as_strided((3, 256), (2 ** 31 + 16, 1))
+    a.copy_(qa[0])
+    assert torch.equal(K.gemm_fp8(a, qa[1], *qb), K.gemm_fp8(*qa, *qb))
+    x, w = rnd(3, 768, seed=1, dtype=BF16), torch.ones(768, device="cuda")
+    xf = far.view(BF16).as_strided((3, 768), (2 ** 30 + 7, 1))
+    xf.copy_(x)
+    assert torch.equal(K.rms_norm_fwd(xf, w, xf)[0], K.rms_norm_fwd(x, w, x)[0])
+    assert torch.equal(K.quant_rows_fp8(xf)[0].view(torch.uint8), K.quant_rows_fp8(x)[0].view(torch.uint8))
+    inv = Fn.rotary_frequencies(64, device="cuda")[0]
+    t = rnd(3, 2, 4, 64, seed=2, dtype=BF16)
+    tf = far.view(BF16).as_strided((3, 2, 4, 64), (2 ** 30, 2 ** 28, 64, 1))
+    tf.copy_(t)
+    want = Fn.rotary(t, None, inv)
+    assert torch.equal(Fn.rotary(tf, None, inv), want)
+    Fn.rotary_(tf, None, inv)
+    assert torch.equal(tf, want)
+
+
 # ----------------------------------------------------------------------------------------------------- together, and around
 def test_the_chain_into_attention():
     """Norm with residual -> 8-bit projection -> rotary in place on the packed queries and keys -> the framework's attention."""
