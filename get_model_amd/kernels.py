@@ -358,16 +358,16 @@ def _refuse(what):
 
 def _on_gpu(*ts):
     """The one GPU of all tensors (None is skipped)."""
-    dev = None
+    index = dev = None
     for t in ts:
         if t is not None:
-            d = t.device
-            if d.type != "cuda":
-                raise RuntimeError("getmi355 kernels need tensors on the GPU (no CPU fallback exists)")
-            if dev is None:
-                dev = d
-            elif d != dev:
-                raise RuntimeError(f"getmi355: tensors on two GPUs ({dev} and {d})")
+            i = t.get_device()
+            if i != index:
+                if i < 0:
+                    raise RuntimeError("getmi355 kernels need tensors on the GPU (no CPU fallback exists)")
+                if index is not None:
+                    raise RuntimeError(f"getmi355: tensors on two GPUs ({dev} and {t.device})")
+                index, dev = i, t.device
     return dev
 
 
@@ -375,8 +375,8 @@ def _rows(t, what):
     """2-D rows of contiguous columns -> distance of the rows in elements (0 for one row that stands for all)."""
     if t.dim() != 2:
         _refuse(f"{what} has to be 2-D (rows of columns), got {tuple(t.shape)}")
-    M, D = t.shape
     ld, step = t.stride()
+    M, D = t.shape
     if step != 1 and D > 1:
         _refuse(f"the columns of {what} have to be contiguous")
     if M > _MOST or D > _MOST:
@@ -507,18 +507,17 @@ def _fp8_operand(q, s, rows, what):
     if q.dtype != FP8 or s.dtype != SCALE:
         _refuse(f"{what} has to be (float8_e4m3fn, float8_e8m0fnu), got ({q.dtype}, {s.dtype})")
     ld = _rows(q, what)
-    cols = q.shape[1]
-    kb = cols // FP8_BLOCK
-    if cols % FP8_BLOCK or kb == 0:
-        _refuse(f"{what} has to be padded to whole blocks of 128 columns, got {cols}")
-    if ld % 16 or q.data_ptr() % 16:
-        _refuse(f"the rows of {what} have to start on 16 bytes")
-    if s.shape != (rows, kb):
-        _refuse(f"the scales of {what} have to be [{rows}, {kb}], got {tuple(s.shape)}")
     lds = _rows(s, "the scales")
+    cols = q.shape[1]
+    if cols & 127 or cols == 0:
+        _refuse(f"{what} has to be padded to whole blocks of 128 columns, got {cols}")
+    if s.shape[0] != rows or s.shape[1] != cols >> 7:
+        _refuse(f"the scales of {what} have to be [{rows}, {cols >> 7}], got {tuple(s.shape)}")
+    if (ld | q.data_ptr()) & 15:
+        _refuse(f"the rows of {what} have to start on 16 bytes")
     if rows <= 1:       # a single row's distance means nothing
         lds = 0
-    if lds % 4 or s.data_ptr() % 4:
+    if (lds | s.data_ptr()) & 3:
         _refuse(f"the scale rows of {what} have to start on 4-byte words")
     return ld, lds
 
