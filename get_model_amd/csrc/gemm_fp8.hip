@@ -118,91 +118,77 @@ template <int N> __device__ __forceinline__ void wait_vm() {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Products too small to fill the chip with 256 x 256 tiles: BM x BN tiles, 4 waves (2 x 2), a ring of three K-tiles of one block
-// (128 bytes a row, the image of the large kernel), two of them in flight, one barrier per K-tile, several workgroups per CU.
-// The scale words (rows of A, then the tile's one block of B) ride in a 1-KiB slot beside each K-tile.
+// Products too small to fill the chip with 256 x 256 tiles: 64 x 64 tiles, 4 waves (2 x 2, 32 x 32 each), a ring of three K-tiles
+// of one block (128 bytes a row, the image of the large kernel), two of them in flight, one barrier per K-tile, three workgroups a
+// CU.  The scale words (64 rows of A, then the tile's one block of B) ride in a 1-KiB slot beside each K-tile.  What bounds it is
+// the CU's path to the caches (16 KiB a K-tile at about 24 bytes a clock), not the depth of the ring: rings of 2, 4 and 6 and tiles
+// of 128 x 64, 64 x 128, 128 x 128, 64 x 32, 32 x 64 and 32 x 32 measured within 10 % or slower over 28 shapes (4020 x 768 x 768:
+// 8.6 us host-bound, 1000 x 2304 x 2304: 15.4).  splits > 1: workgroup (tile, s) takes the s-th part of the depth.
 // ------------------------------------------------------------------------------------------------
-// wait until at most n K-tiles (OPS operations each) are in flight, n <= MAX
-template <int OPS, int MAX> __device__ __forceinline__ void wait_tiles(int n) {
-    if constexpr (MAX == 0) wait_vm<0>();
-    else if (n >= MAX) wait_vm<MAX * OPS>();
-    else wait_tiles<OPS, MAX - 1>(n);
-}
+constexpr int T64_SLOTS = 3, T64_STAGE = 128 * 128 + 1024, T64_OPS = 5;      // LDS-DMA operations a wave and K-tile
 
-template <int BM, int BN, int S>
 __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws) {
-    constexpr int STAGE = (BM + BN) * 128 + 1024, OPS = (BM + BN) / 32 + 1, MT = BM / 32, NT = BN / 32;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1, nkb = p.K >> 7;
-    const int tiles_n = (p.N + BN - 1) / BN, bid = xcd_remap(blockIdx.x, gridDim.x), lid = bid / splits, sp = bid - lid * splits;
-    const int tm = lid / tiles_n, tn = lid - tm * tiles_n;
+    const int tiles_n = (p.N + 63) / 64, bid = xcd_remap(blockIdx.x, gridDim.x), lid = bid / splits, sp = bid - lid * splits;
+    const int tm = lid / tiles_n, tn = lid - tm * tiles_n, m0 = tm * 64, n0 = tn * 64;
     const int kb0 = (int)((int64_t)nkb * sp / splits), nk = (int)((int64_t)nkb * (sp + 1) / splits) - kb0;      // >= 1: splits <= nkb
-    const int m0 = tm * BM, n0 = tn * BN;
     // 16-byte pieces: wave w's i-th instruction moves rows 8 (4 i + w) .. + 7 of the [A; B] image
-    const unsigned char* src[OPS - 1];
+    const unsigned char* src[4];
 #pragma unroll
-    for (int i = 0; i < OPS - 1; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int row = (i * 4 + wave) * 8 + (lane >> 3), chunk = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
-        src[i] = (row < BM ? p.A + (size_t)min(m0 + row, p.M - 1) * p.lda : p.B + (size_t)min(n0 + row - BM, p.N - 1) * p.ldb) + chunk;
+        src[i] = (row < 64 ? p.A + (size_t)min(m0 + row, p.M - 1) * p.lda : p.B + (size_t)min(n0 + row - 64, p.N - 1) * p.ldb) + chunk;
     }
-    const unsigned char* ssrc = tid < BM ? p.sa + (size_t)min(m0 + tid, p.M - 1) * p.lsa : p.sb + (size_t)(n0 >> 7) * p.lsb;
+    const unsigned char* ssrc = tid < 64 ? p.sa + (size_t)min(m0 + tid, p.M - 1) * p.lsa : p.sb + (size_t)(n0 >> 7) * p.lsb;
     auto issue = [&](int k, int slot) {
-        char* b = smem + slot * STAGE;
+        char* b = smem + slot * T64_STAGE;
 #pragma unroll
-        for (int i = 0; i < OPS - 1; ++i) glds16(src[i] + (size_t)(kb0 + k) * 128, b + (i * 4 + wave) * 1024);
-        glds4(ssrc + ((kb0 + k) & ~3), b + (BM + BN) * 128 + wave * 256);
+        for (int i = 0; i < 4; ++i) glds16(src[i] + (size_t)(kb0 + k) * 128, b + (i * 4 + wave) * 1024);
+        glds4(ssrc + ((kb0 + k) & ~3), b + 128 * 128 + wave * 256);
     };
-    f32x4 acc[MT][NT];
+    f32x4 acc[2][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int fsw = (r >> 1) & 7;
     const unsigned lds0 = lds_addr(smem), off0 = r * 128 + ((c ^ fsw) << 4), off1 = r * 128 + (((4 + c) ^ fsw) << 4);
-#pragma unroll
-    for (int k = 0; k < S - 1; ++k)
-        if (k < nk) issue(k, k);
+    issue(0, 0);
+    if (nk > 1) issue(1, 1);
     int slot = 0;
     for (int k = 0; k < nk; ++k) {
-        wait_tiles<OPS, S - 2>(nk - 1 - k);      // K-tile k has landed (this wave's share); the S - 2 after it stay in flight
-        phase_barrier();                          // ... every wave's share; and K-tile k - 1 has been read by all
-        if (k + S - 1 < nk) issue(k + S - 1, slot == 0 ? S - 1 : slot - 1);
-        const unsigned b = lds0 + slot * STAGE, ab = b + wm * (BM / 2) * 128, bb = b + (BM + wn * (BN / 2)) * 128, sc = b + (BM + BN) * 128;
-        u32x4 fa[MT][2], fb[NT][2];
-        unsigned sa[MT], sb;
-        // (inline asm: hipcc would wait for every LDS-DMA in flight before a read it can see)
-        asm volatile("ds_read_b32 %0, %1" : "=&v"(sb) : "v"(sc + (BM < 256 ? BM * 4 : 0)) : "memory");
-#pragma unroll
-        for (int i = 0; i < MT; ++i) asm volatile("ds_read_b32 %0, %1 offset:%2" : "=&v"(sa[i]) : "v"(sc + (wm * (BM / 2) + r) * 4), "n"(i * 64) : "memory");
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fa[i][0]) : "v"(ab + off0), "n"(i * 2048) : "memory");
-            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fa[i][1]) : "v"(ab + off1), "n"(i * 2048) : "memory");
-        }
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fb[j][0]) : "v"(bb + off0), "n"(j * 2048) : "memory");
-            asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fb[j][1]) : "v"(bb + off1), "n"(j * 2048) : "memory");
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(sb) : : "memory");
-#pragma unroll
-        for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(sa[i]), "+v"(fa[i][0]), "+v"(fa[i][1]));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(fb[j][0]), "+v"(fb[j][1]));
+        if (k + 1 < nk) wait_vm<T64_OPS>(); else wait_vm<0>();      // K-tile k has landed (this wave's share), k + 1 stays in flight
+        phase_barrier();                                              // ... every wave's share; and K-tile k - 1 has been read by all
+        if (k + 2 < nk) issue(k + 2, slot == 0 ? 2 : slot - 1);
+        const unsigned b = lds0 + slot * T64_STAGE, ab = b + wm * 4096, bb = b + 8192 + wn * 4096, sc = b + 128 * 128;
+        const unsigned a0 = ab + off0, a1 = ab + off1, b0 = bb + off0, b1 = bb + off1;
+        u32x4 fa[2][2], fb[2][2];
+        unsigned sa[2], sb;
+        // (inline asm, reads and wait in one statement: hipcc would wait for every LDS-DMA in flight before a read it can see)
+        asm volatile(
+            "ds_read_b32 %0, %11 offset:256\n\tds_read_b32 %1, %12\n\tds_read_b32 %2, %12 offset:64\n\t"
+            "ds_read_b128 %3, %13\n\tds_read_b128 %4, %14\n\tds_read_b128 %5, %13 offset:2048\n\tds_read_b128 %6, %14 offset:2048\n\t"
+            "ds_read_b128 %7, %15\n\tds_read_b128 %8, %16\n\tds_read_b128 %9, %15 offset:2048\n\tds_read_b128 %10, %16 offset:2048\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(sb), "=&v"(sa[0]), "=&v"(sa[1]), "=&v"(fa[0][0]), "=&v"(fa[0][1]), "=&v"(fa[1][0]), "=&v"(fa[1][1]), "=&v"(fb[0][0]),
+              "=&v"(fb[0][1]), "=&v"(fb[1][0]), "=&v"(fb[1][1])
+            : "v"(sc), "v"(sc + (wm * 32 + r) * 4), "v"(a0), "v"(a1), "v"(b0), "v"(b1)
+            : "memory");
         const int sh = ((kb0 + k) & 3) * 8;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < 2; ++j)
                 acc[i][j] = mfma_fp8(join8(fb[j][0], fb[j][1]), join8(fa[i][0], fa[i][1]), acc[i][j], (int)(sb >> sh), (int)(sa[i] >> sh));
-        slot = slot == S - 1 ? 0 : slot + 1;
+        slot = slot == 2 ? 0 : slot + 1;
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int m = m0 + wm * (BM / 2) + i * 16 + r, n = n0 + wn * (BN / 2) + j * 16 + c * 4;
+        for (int j = 0; j < 2; ++j) {
+            const int m = m0 + wm * 32 + i * 16 + r, n = n0 + wn * 32 + j * 16 + c * 4;
             if (splits == 1) store_out4(p, m, n, acc[i][j], gran);
             else if (m < p.M && n < p.N) *reinterpret_cast<f32x4*>(ws + ((size_t)sp * p.M + m) * ((p.N + 3) & ~3) + n) = acc[i][j];
         }
@@ -232,6 +218,13 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Fp8Args p, int gran,
 // 32 rows of A (lanes 0-31) and of the wave's own 128-column block of B (lanes 32-63).  The words are read at every fourth K-tile
 // and shifted down a byte in between; the matrix unit takes the low byte.
 // Stores are exactly E per wave and tile (inline asm, bounds-checked), so the next tile's counted waits leave them in flight.
+//
+// Measured (warm, 3 operands in rotation): 8192^3 407 us (2.70 PFLOP/s; the library's product with one scale per tensor 410),
+// 16384 x 4096 x 4096 206 us (2.66), 51456 x 2304 x 768 99 us (1.85).  What bounds it is the CU's one path to the caches, 64 KiB a
+// K-tile in and the tile out, at 16 - 20 bytes a clock (counters: matrix units 65 % busy at 8192^3, LDS 26 %, bank conflicts 2 %):
+// 51456 x 2304 x 768 carries 948 MB over it.  Tried without gain: wave priorities around the matrix instructions, reads before the
+// next half-tile's issue, two launches of different tile height against the partial last round, other tile orders, a K order turned
+// per XCD; output stores through the cache instead of past it: 110 -> 116 us.
 // ------------------------------------------------------------------------------------------------
 #define F8_SCALES 131072
 #define F8_BIAS (F8_SCALES + 2 * 2048)
@@ -594,9 +587,8 @@ template <int MT, int NT> static int launch_rows(const Fp8Args& p, int gran, hip
     return GETMI_OK;
 }
 static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStream_t st) {
-    constexpr int S = 3, lds = S * (128 * 128 + 1024);
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
-    hipLaunchKernelGGL((gemm_fp8_tile_kernel<64, 64, S>), dim3((unsigned)(tiles * splits)), dim3(256), lds, st, p, gran, splits, ws);
+    hipLaunchKernelGGL(gemm_fp8_tile_kernel, dim3((unsigned)(tiles * splits)), dim3(256), T64_SLOTS * T64_STAGE, st, p, gran, splits, ws);
     if (splits > 1) {
         const int64_t blocks = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
         hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p, gran, splits,

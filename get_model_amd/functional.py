@@ -19,7 +19,6 @@ import os
 import weakref
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 
@@ -826,6 +825,13 @@ class FusedLoss(torch.autograd.Function):
 
 # --------------------------------------------------------------------------------------------
 # Operators of encoders that normalise by the root mean square, rotate queries and keys by position and serve in 8 bits.
+def _first_order_only(what):
+    # (torch's once_differentiable looks at the incoming gradients alone: where those need none, as under a sum, it hands out first
+    #  derivatives that are silently constant in the inputs)
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"get_model_amd: {what} has no second derivative; take its gradient without create_graph")
+
+
 class _RMSNorm(torch.autograd.Function):
     """y = w * h * rstd, h = x + residual.  Saves h as it is stored (in the residual's type) and the fp32 rstd of the unrounded sum."""
 
@@ -840,8 +846,8 @@ class _RMSNorm(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
+        _first_order_only("rms_norm")
         h, rstd, weight = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         xt, rt = ctx.types
@@ -849,8 +855,8 @@ class _RMSNorm(torch.autograd.Function):
             return (dh.to(xt) if need_x and dh is not None else None, torch.zeros_like(weight) if need_w else None,
                     dh if need_r else None, None, None)
         other = need_x and rt is not None and rt != xt      # a bf16 branch on an fp32 stream
-        dx, dx2, dw = K.rms_norm_bwd(dy.contiguous(), h, rstd, weight, None if dh is None else dh.contiguous(), want_dw=need_w,
-                                     bf16_copy=other)
+        dx, dx2, dw = K.rms_norm_bwd_unchecked(dy.contiguous(), h, rstd, weight, None if dh is None else dh.contiguous(), need_w, other,
+                                               h.device)
         return (dx2 if other else dx) if need_x else None, dw, dx if need_r else None, None, None
 
 
@@ -985,15 +991,15 @@ class _Rotary(torch.autograd.Function):
         return q if k is None else (q, k)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk=None):
+        _first_order_only("rotary")
         inv_freq, positions = ctx.saved_tensors
         dq, dk = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
-        if dq is None:
-            out = (None, None if dk is None else K.rotary(dk, None, inv_freq, positions, *ctx.rest, backward=True)[0])
-        else:
-            out = K.rotary(dq, dk, inv_freq, positions, *ctx.rest, backward=True)
-        return out + (None,) * 5
+        if dq is None and dk is None:
+            return (None,) * 7
+        first, second = (dk, None) if dq is None else (dq, dk)
+        out = K.rotary_unchecked(first, second, inv_freq, positions, *ctx.rest, True, False, inv_freq.device)
+        return (out if dq is not None else (None, out[0])) + (None,) * 5
 
 
 def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.0):

@@ -4,6 +4,7 @@ torch is used only to allocate device buffers and to provide the stream; all ari
 libgetmi355.so.  Every function requires CUDA(HIP) tensors and raises RuntimeError otherwise.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -426,7 +427,7 @@ def rms_norm_fwd(x, weight, residual=None, eps=1e-6, out_dtype=BF16, want_rstd=F
 def rms_norm_bwd(dy, h, rstd, weight, dh=None, want_dw=True, bf16_copy=False):
     """-> (dx, dx2, dw).  dy fp32 / bf16 [M,D], h [M,D] (what was normalised; rows may lie apart), dh of h's type or None.
     dx in h's type is the gradient of x and of the residual alike; dx2 is dx in bf16 (only with bf16_copy and an fp32 h)."""
-    ldh = _rows(h, "h")
+    _rows(h, "h")
     M, D = h.shape
     if dy.shape != h.shape or dy.dtype not in _TYPE or not dy.is_contiguous():
         _refuse("dy has to be contiguous float32 or bfloat16 of h's shape")
@@ -440,16 +441,30 @@ def rms_norm_bwd(dy, h, rstd, weight, dh=None, want_dw=True, bf16_copy=False):
         _refuse("dh has to be contiguous, of h's shape and type")
     if bf16_copy and h.dtype != F32:
         _refuse("a bf16 copy of dx is made next to an fp32 one only")
-    dev = _on_gpu(dy, h, rstd, weight, dh)
+    return rms_norm_bwd_unchecked(dy, h, rstd, weight, dh, want_dw, bf16_copy, _on_gpu(dy, h, rstd, weight, dh))
+
+
+@functools.lru_cache(maxsize=256)
+def _rms_norm_bwd_workspace(M, D):
+    return max(lib.query("getmi_rmsnorm_bwd_workspace_bytes", M, D), 256)
+
+
+def rms_norm_bwd_unchecked(dy, h, rstd, weight, dh, want_dw, bf16_copy, dev):
+    """rms_norm_bwd for a caller that knows its arguments to be right (functional: what the forward saved, autograd's gradients)."""
+    M, D = h.shape
     dx = torch.empty(M, D, dtype=h.dtype, device=dev)
     dx2 = torch.empty(M, D, dtype=BF16, device=dev) if bf16_copy else None
     if M == 0:
         return dx, dx2, torch.zeros(D, dtype=F32, device=dev) if want_dw else None
-    dw = torch.empty(D, dtype=F32, device=dev) if want_dw else None
-    ws = _ws(lib.query("getmi_rmsnorm_bwd_workspace_bytes", M, D), dev) if want_dw else None
-    lib.launch("getmi_rmsnorm_bwd", dev, dy.data_ptr(), _TYPE[dy.dtype], h.data_ptr(), _TYPE[h.dtype], ldh, rstd.data_ptr(),
+    dw = ws = None
+    need = 0
+    if want_dw:
+        need = _rms_norm_bwd_workspace(M, D)
+        dw = torch.empty(D, dtype=F32, device=dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    lib.launch("getmi_rmsnorm_bwd", dev, dy.data_ptr(), _TYPE[dy.dtype], h.data_ptr(), _TYPE[h.dtype], h.stride(0), rstd.data_ptr(),
                weight.data_ptr(), None if dh is None else dh.data_ptr(), dx.data_ptr(), None if dx2 is None else dx2.data_ptr(),
-               None if dw is None else dw.data_ptr(), M, D, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+               None if dw is None else dw.data_ptr(), M, D, None if ws is None else ws.data_ptr(), need)
     return dx, dx2, dw
 
 
@@ -592,7 +607,6 @@ def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.
     if q.dim() != 4:
         _refuse(f"q has to be [B, T, heads, D], got {tuple(q.shape)}")
     B, T, Hq, D = q.shape
-    qb, qt, qh, step = q.stride()
     dtype = q.dtype
     if dtype not in _TYPE:
         _refuse(f"q has to be float32 or bfloat16, got {dtype}")
@@ -603,46 +617,56 @@ def rotary(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1.
     R = 2 * inv_freq.shape[0]
     if not 0 < R <= min(D, 2048):
         _refuse(f"{R} rotated columns do not fit heads of {D} (at most 2048)")
-    if step != 1 and D > 1:
+    if q.stride(3) != 1 and D > 1:
         _refuse("the columns of q have to be contiguous")
-    Hk = kb = kt = kh = 0
+    Hk = 0
     if k is not None:
         if k.dim() != 4 or k.dtype != dtype or k.shape[0] != B or k.shape[1] != T or k.shape[3] != D:
             _refuse(f"k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {dtype}")
         Hk = k.shape[2]
-        kb, kt, kh, step = k.stride()
-        if step != 1 and D > 1:
+        if k.stride(3) != 1 and D > 1:
             _refuse("the columns of k have to be contiguous")
     if B * T > _MOST or Hq + Hk > 65536:
         _refuse(f"at most {_MOST} tokens and 65536 heads, got {B * T} and {Hq + Hk}")
     if not -2 ** 53 < offset < 2 ** 53:
         _refuse(f"offset {offset} is not below 2^53")
-    pb = pt = wide = 0
     if positions is not None:
         if positions.dtype != torch.int64 and positions.dtype != torch.int32:
             _refuse(f"positions have to be int64 or int32, got {positions.dtype}")
         if offset != 0:
             _refuse("positions and an offset exclude each other")
-        wide = int(positions.dtype == torch.int64)
-        if positions.shape == (B, T):
-            pb, pt = positions.stride()
-        elif positions.shape == (T,):
-            pt = positions.stride(0)
-        else:
+        if positions.shape != (B, T) and positions.shape != (T,):
             _refuse(f"positions have to be [{B}, {T}] or [{T}], got {tuple(positions.shape)}")
+    if inplace and (_overlaps(q) or (k is not None and (_overlaps(k) or _share(q, k)))):
+        _refuse("in place needs tensors whose elements do not share memory")
+    return rotary_unchecked(q, k, inv_freq, positions, offset, layout, magnitude, backward, inplace, _on_gpu(q, k, inv_freq, positions))
+
+
+def rotary_unchecked(q, k, inv_freq, positions, offset, layout, magnitude, backward, inplace, dev):
+    """rotary for a caller that knows its arguments to be right."""
+    B, T, Hq, D = q.shape
+    qb, qt, qh, _ = q.stride()
+    dtype = q.dtype
+    Hk = kb = kt = kh = pb = pt = wide = 0
+    qo, ko = q, k
+    if k is not None:
+        Hk = k.shape[2]
+        kb, kt, kh, _ = k.stride()
+    if positions is not None:
+        wide = int(positions.dtype == torch.int64)
+        if positions.dim() == 2:
+            pb, pt = positions.stride()
+        else:
+            pt = positions.stride(0)
     if inplace:
-        if _overlaps(q) or (k is not None and (_overlaps(k) or _share(q, k))):
-            _refuse("in place needs tensors whose elements do not share memory")
-        dev = _on_gpu(q, k, inv_freq, positions)
-        qo, ko = q, k
         strides = _Strides(qb, qt, qh, qb, qt, qh, kb, kt, kh, kb, kt, kh)
     else:
-        dev = _on_gpu(q, k, inv_freq, positions)
         qo = torch.empty(B, T, Hq, D, dtype=dtype, device=dev)
-        ko = None if k is None else torch.empty(B, T, Hk, D, dtype=dtype, device=dev)
+        if k is not None:
+            ko = torch.empty(B, T, Hk, D, dtype=dtype, device=dev)
         strides = _Strides(qb, qt, qh, T * Hq * D, Hq * D, D, kb, kt, kh, T * Hk * D, Hk * D, D)
     if B * T * (Hq + Hk):
         lib.launch("getmi_rotary", dev, q.data_ptr(), qo.data_ptr(), Hq, None if k is None else k.data_ptr(),
-                   None if k is None else ko.data_ptr(), Hk, strides, _TYPE[dtype], B, T, D, R, inv_freq.data_ptr(),
+                   None if k is None else ko.data_ptr(), Hk, strides, _TYPE[dtype], B, T, D, 2 * inv_freq.shape[0], inv_freq.data_ptr(),
                    None if positions is None else positions.data_ptr(), wide, pb, pt, offset, layout == "interleaved", backward, magnitude)
     return qo, ko

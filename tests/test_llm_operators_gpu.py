@@ -623,3 +623,13 @@ def test_the_same_call_twice_is_the_same():
     assert all(torch.equal(u, v) for u, v in zip(a, b))
     qa, qb = operands(3, 300, 8192)
     assert torch.equal(K.gemm_fp8(*qa, *qb), K.gemm_fp8(*qa, *qb))
+
+
+def test_no_second_derivative_in_silence():
+    """A backward pass that is itself to be differentiated is refused: its gradients would be constants."""
+    x, w = rnd(4, 96, seed=1).requires_grad_(), torch.ones(96, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(Fn.rms_norm(x, w, out_dtype=F32).sum(), x, create_graph=True)
+    q = rnd(1, 3, 2, 8, seed=2).requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(Fn.rotary(q, None, Fn.rotary_frequencies(8, device="cuda")[0]).square().sum(), q, create_graph=True)
