@@ -9,6 +9,12 @@
 // weight gradient are formed in fp32; y is formed from the unrounded fp32 h, and h is rounded once, to the residual's type.
 // A power-of-two scale makes y / scale exact, so q carries the one rounding of the format itself, and it is what the
 // matrix unit's own block scaling takes (gemm_fp8.hip).
+//
+// Measured, 51456 x 768, bf16 x on an fp32 residual, three operand sets in rotation (a 1-GiB copy reaches 5.0 TB/s): forward 72 us
+// (12 bytes an element: 6.6 TB/s, part of it out of the Infinity Cache), 8-bit 71 us, backward 102 us (16 bytes, 6.2 TB/s) + 5 for
+// the column sums' second stage.  Odd width, 51456 x 283 fp32: 20 / 35 us.  One row of 768: 2.1 us.  What got it there: the next
+// row's loads in flight while a row is summed (94 -> 80), element-aligned wide accesses instead of single ones for odd widths (36 ->
+// 20), nt loads for what the caches cannot hold, 1024 workgroups forward / 512 backward.
 #include "common.h"
 
 namespace {

@@ -7,6 +7,10 @@
 // 3e-9 for the sine and 2e-9 for the cosine).  A workgroup forms the R/2 cosines and sines of its few tokens once, in LDS, so
 // the 64-bit work is a small fraction and every head reads them back; q and k share one launch.  HBM-bound: every element is
 // read once and written once, 16 bytes per lane.
+//
+// Measured (a 1-GiB copy reaches 5.0 TB/s): 256 x 201 x 24 heads of 64 bf16, half: 63 us (316 MB, 5.0 TB/s), in place 69;
+// 32768 x 18 x 128 fp32, interleaved, half of the head turned: 115 us (604 MB, 5.3 TB/s); 64 single tokens: 3.4 us.  With one piece in
+// flight per lane, a division per piece and copying lanes behind rotating ones it was 75 and 157 us.
 #include "common.h"
 
 namespace {
