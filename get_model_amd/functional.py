@@ -1018,4 +1018,7 @@ def rotary_(q, k, inv_freq, positions=None, offset=0, layout="half", magnitude=1
     """rotary in place, for inference: q and k (or the head range of a packed projection that holds both: k None) are overwritten."""
     _no_grad_only("rotary_", q, k)
     q, k = K.rotary(q, k, inv_freq, positions, offset, layout, magnitude, inplace=True)
+    for t in (q, k):      # a graph that saved the old values has to notice
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
     return q if k is None else (q, k)

@@ -532,8 +532,8 @@ def _fp8_operand(q, s, rows, what):
         _refuse(f"the rows of {what} have to start on 16 bytes")
     if rows <= 1:       # a single row's distance means nothing
         lds = 0
-    if (lds | s.data_ptr()) & 3:
-        _refuse(f"the scale rows of {what} have to start on 4-byte words")
+    if (lds | s.data_ptr()) & 3 or lds > _MOST:
+        _refuse(f"the scale rows of {what} have to start on 4-byte words, less than 2 GiB apart")
     return ld, lds
 
 

@@ -625,6 +625,46 @@ def test_the_same_call_twice_is_the_same():
     assert torch.equal(K.gemm_fp8(*qa, *qb), K.gemm_fp8(*qa, *qb))
 
 
+def test_one_tensor_in_two_places():
+    """The same tensor as input and residual, as both operands' leaves; gradients that share no memory."""
+    w = 1 + 0.1 * rnd(96, seed=1)
+    x = rnd(5, 96, seed=2).requires_grad_()
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    dy, dh = rnd(5, 96, seed=3), rnd(5, 96, seed=4)
+    torch.autograd.backward(Fn.rms_norm(x, w, x, out_dtype=F32), (dy, dh))
+    torch.autograd.backward(Fn.rms_norm(a, w, b, out_dtype=F32), (dy, dh))
+    assert torch.equal(a.grad, b.grad) and torch.equal(x.grad, a.grad + b.grad)
+    a.grad.add_(1)
+    assert not torch.equal(a.grad, b.grad)
+    # twice through the same weight: its gradient is the sum
+    wl = w.clone().requires_grad_()
+    y1, y2 = Fn.rms_norm(a.detach(), wl, out_dtype=F32), Fn.rms_norm(dh, wl, out_dtype=F32)
+    one, two = (torch.autograd.grad(y, wl, dy, retain_graph=True)[0] for y in (y1, y2))
+    assert torch.equal(torch.autograd.grad((y1, y2), wl, (dy, dy))[0], one + two)
+    q = rnd(1, 4, 2, 8, seed=5).requires_grad_()
+    inv = Fn.rotary_frequencies(8, device="cuda")[0]
+    g = rnd(1, 4, 2, 8, seed=6)
+    both = torch.autograd.grad(Fn.rotary(q, q, inv), q, (g, g))[0]
+    assert torch.equal(both, 2 * torch.autograd.grad(Fn.rotary(q, None, inv), q, g)[0])
+    # one buffer as both operands, one row of scales for all rows
+    e = K.quant_blocks_fp8(rnd(128, 256, seed=7))
+    gram = K.gemm_fp8(e[0], e[1].expand(128, 2), *e)
+    assert torch.equal(gram, gram.t())
+
+
+def test_values_that_a_graph_saved_are_not_overwritten_in_silence():
+    x = rnd(1, 4, 2, 8, seed=1)
+    w = rnd(1, 4, 2, 8, seed=2).requires_grad_()
+    out = (x * w).sum()                     # saves x
+    with torch.no_grad():
+        Fn.rotary_(x, None, Fn.rotary_frequencies(8, device="cuda")[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+    with torch.inference_mode():
+        t = torch.ones(1, 4, 2, 8, device="cuda")
+        Fn.rotary_(t, None, Fn.rotary_frequencies(8, device="cuda")[0])
+
+
 def test_no_second_derivative_in_silence():
     """A backward pass that is itself to be differentiated is refused: its gradients would be constants."""
     x, w = rnd(4, 96, seed=1).requires_grad_(), torch.ones(96, device="cuda", requires_grad=True)
