@@ -25,7 +25,7 @@ FLAGS += os.environ.get("GETMI_EXTRA_HIPCC_FLAGS", "").split()      # experiment
 
 def _stamp(src):
     h = hashlib.sha1()
-    for f in [src, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_pipe.h"), os.path.join(HERE, "..", "include", "getmi355.h")]:
+    for f in [src, os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_pipe.h"), os.path.join(CSRC, "fp8.h"), os.path.join(HERE, "..", "include", "getmi355.h")]:
         with open(f, "rb") as fh:
             h.update(fh.read())
     h.update(" ".join(FLAGS).encode())

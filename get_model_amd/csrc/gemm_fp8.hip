@@ -1,6 +1,7 @@
 // out[M,N] (bf16) = sum over blocks b of 128 columns:  2^sa[m,b] * 2^sb[n/128,b] * sum_{k in b} A[m,k] * B[n,k]   (+ bias[n])
 // with e4m3 operands.  v_mfma_scale_f32_16x16x128_f8f6f4 takes one block of 128 in its depth and applies one power-of-two scale
 // per row and 32 columns by itself, so the scales cost no vector instruction and the accumulators are plain fp32 sums.
+#include "fp8.h"
 #include "gemm_pipe.h"
 #include <atomic>
 #include <type_traits>
@@ -9,7 +10,7 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 struct Fp8Args {
     const unsigned char* A; const unsigned char* sa; const unsigned char* B; const unsigned char* sb; const float* bias; bf16_t* out;
-    size_t lda, ldb, ldo; int lsa, lsb, M, N, K;
+    size_t lda, ldb, ldo; int lsa, lsb, M, N, K, Ka;
 };
 
 __device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
@@ -49,7 +50,64 @@ __device__ __forceinline__ void store_out4(const Fp8Args& p, int m, int n, f32x4
 // and the W partial sums are joined in LDS in a fixed order.  The B rows are the matrix unit's rows and the A rows its columns, so
 // a lane ends up with four consecutive n of one m.
 // ------------------------------------------------------------------------------------------------
-template <int MT, int NT>
+enum { A_F32 = 0, A_BF16 = 1, A_FP8 = 2 };
+
+// Sixteen consecutive columns of a 16- or 32-bit row, of which n exist (the others are zero).  Rows may start on any element.
+template <int AT> struct Sixteen { float v[16]; };
+template <int AT> __device__ __forceinline__ Sixteen<AT> load16(const unsigned char* row, int col, int n) {
+    Sixteen<AT> s;
+    if constexpr (AT == A_BF16) {
+        typedef __attribute__((ext_vector_type(8), aligned(2))) unsigned short us8;
+        const bf16_t* p = reinterpret_cast<const bf16_t*>(row) + col;
+        if (n >= 16) {
+            const us8 x = *reinterpret_cast<const us8*>(p), y = *reinterpret_cast<const us8*>(p + 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { s.v[i] = bf2f(x[i]); s.v[8 + i] = bf2f(y[i]); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s.v[i] = i < n ? bf2f(p[i]) : 0.f;
+        }
+    } else {
+        typedef __attribute__((ext_vector_type(4), aligned(4))) float f4;
+        const float* p = reinterpret_cast<const float*>(row) + col;
+        if (n >= 16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 x = reinterpret_cast<const f4*>(p)[i];
+                s.v[4 * i] = x[0]; s.v[4 * i + 1] = x[1]; s.v[4 * i + 2] = x[2]; s.v[4 * i + 3] = x[3];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s.v[i] = i < n ? p[i] : 0.f;
+        }
+    }
+    return s;
+}
+// A lane's 32 values of one block of its row, quantised on the way: the block's maximum is the maximum over the four lanes that hold
+// it (16 and 32 apart).  The same values and scale as the row quantiser's.
+template <int AT> __device__ __forceinline__ i32x8 frag_quantised(const unsigned char* row, int kb, int c, int K, unsigned& scale) {
+    const int col = kb * 128 + c * 16;
+    const Sixteen<AT> lo = load16<AT>(row, col, K - col), hi = load16<AT>(row, col + 64, K - col - 64);
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, max(abs_bits(lo.v[i]), abs_bits(hi.v[i])));
+    m = max(m, (unsigned)__builtin_amdgcn_ds_swizzle((int)m, 0x401f));
+    m = max(m, (unsigned)__shfl_xor((int)m, 32, 64));
+    scale = scale_byte(m);
+    const float inv = inv_scale(scale);
+    const bool finite = m < 0x7f800000u;
+    i32x8 f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[i] = (int)pack4fp8(lo.v[4 * i], lo.v[4 * i + 1], lo.v[4 * i + 2], lo.v[4 * i + 3], inv, finite);
+        f[4 + i] = (int)pack4fp8(hi.v[4 * i], hi.v[4 * i + 1], hi.v[4 * i + 2], hi.v[4 * i + 3], inv, finite);
+    }
+    return f;
+}
+
+// AT: e4m3 rows with scales, or 16- / 32-bit rows (p.sa unused, p.lda in bytes, p.Ka columns) that every workgroup quantises for
+// itself: one launch for a token's linear.
+template <int MT, int NT, int AT>
 __global__ __launch_bounds__(1024) void gemm_fp8_rows_kernel(Fp8Args p, int gran) {
     extern __shared__ __attribute__((aligned(16))) f32x4 part[];      // [W][NT * MT][64]
     const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
@@ -61,8 +119,8 @@ __global__ __launch_bounds__(1024) void gemm_fp8_rows_kernel(Fp8Args p, int gran
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
         const size_t m = min(m0 + j * 16 + r, p.M - 1);
-        a[j] = p.A + m * p.lda + c * 16;
-        sa[j] = p.sa + m * p.lsa;
+        a[j] = p.A + m * p.lda + (AT == A_FP8 ? c * 16 : 0);
+        sa[j] = p.sa + (AT == A_FP8 ? m * p.lsa : 0);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -79,13 +137,18 @@ __global__ __launch_bounds__(1024) void gemm_fp8_rows_kernel(Fp8Args p, int gran
             const int k = kb + u * W;
 #pragma unroll
             for (int i = 0; i < NT; ++i) fb[u][i] = frag_global(b[i] + (size_t)k * 128);
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                fa[u][j] = frag_global(a[j] + (size_t)k * 128);
-                xa[u][j] = sa[j][k];
-            }
             xb[u] = *reinterpret_cast<const unsigned*>(sb + (k & ~3)) >> ((k & 3) * 8);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                const int k = kb + u * W;
+                if constexpr (AT == A_FP8) {
+                    fa[u][j] = frag_global(a[j] + (size_t)k * 128);
+                    xa[u][j] = sa[j][k];
+                } else fa[u][j] = frag_quantised<AT>(a[j], k, c, p.Ka, xa[u][j]);
+            }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -93,7 +156,7 @@ __global__ __launch_bounds__(1024) void gemm_fp8_rows_kernel(Fp8Args p, int gran
 #pragma unroll
                 for (int j = 0; j < MT; ++j) acc[i][j] = mfma_fp8(fb[u][i], fa[u][j], acc[i][j], (int)xb[u], (int)xa[u][j]);
     };
-    constexpr int U = MT * NT <= 2 ? 4 : 2;
+    constexpr int U = MT * NT > 2 || AT != A_FP8 ? 2 : 4;
     int kb = wave;
     for (; kb + (U - 1) * W < nkb; kb += U * W) step(std::integral_constant<int, U>{}, kb);
     for (; kb < nkb; kb += W) step(std::integral_constant<int, 1>{}, kb);
@@ -578,10 +641,10 @@ template <int GR> static int launch_big(const Fp8Args& p, hipStream_t st) {
     return best == 4 ? launch_256p<4, GR>(p, st) : best == 3 ? launch_256p<3, GR>(p, st) : launch_256p<2, GR>(p, st);
 }
 
-template <int MT, int NT> static int launch_rows(const Fp8Args& p, int gran, hipStream_t st) {
+template <int MT, int NT, int AT = A_FP8> static int launch_rows(const Fp8Args& p, int gran, hipStream_t st) {
     const int nkb = p.K / 128, wgs = ((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
     const int W = nkb >= 32 && wgs <= 256 ? 16 : nkb >= 16 ? 8 : 4;      // 4, 8 and 16 measure alike where either applies
-    hipLaunchKernelGGL((gemm_fp8_rows_kernel<MT, NT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * W),
+    hipLaunchKernelGGL((gemm_fp8_rows_kernel<MT, NT, AT>), dim3((p.N + 16 * NT - 1) / (16 * NT), (p.M + 16 * MT - 1) / (16 * MT)), dim3(64 * W),
                        (size_t)W * MT * NT * 1024, st, p, gran);
     GETMI_CHECK_LAUNCH("gemm_fp8");
     return GETMI_OK;
@@ -641,7 +704,7 @@ int getmi_gemm_fp8_impl(const void* A, const void* sa, const void* B, const void
                     "gemm_fp8: scale rows have to start on 4 bytes");
     GETMI_CHECK_ARG((int64_t)((M + 63) / 64) * ((N + 63) / 64) < 0x7fffffff, "gemm_fp8: M=%d N=%d too large", M, N);
     Fp8Args p{(const unsigned char*)A, (const unsigned char*)sa, (const unsigned char*)B, (const unsigned char*)sb, bias, (bf16_t*)out,
-              (size_t)lda, (size_t)ldb, (size_t)ldo, lsa, lsb, M, N, K};
+              (size_t)lda, (size_t)ldb, (size_t)ldo, lsa, lsb, M, N, K, K};
     const int gran = granularity(out, N, ldo);
     const size_t lim = 0xF0000000ull;      // the large kernel addresses each operand with 32 bits
     const bool fits = (size_t)M * lda < lim && (size_t)N * ldb < lim && (size_t)M * ldo * 2 < lim && (size_t)M * lsa < lim && (size_t)N * lsb < lim;
@@ -653,4 +716,18 @@ int getmi_gemm_fp8_impl(const void* A, const void* sa, const void* B, const void
     if (pl.kind == ROWS21) return launch_rows<2, 1>(p, gran, st);
     if (pl.kind == BIG && fits) return gran == 8 ? launch_big<8>(p, st) : gran >= 2 ? launch_big<2>(p, st) : launch_big<1>(p, st);
     return launch_tile(p, gran, pl.splits, (float*)workspace, st);
+}
+
+// Up to 16 rows of fp32 / bf16, quantised inside the product: x[M, K] (rows ldx elements apart), B[N, Kp] and its scales as above.
+int getmi_linear_fp8_rows_impl(const void* x, int xt, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M, int N,
+                               int K, int64_t ldb, int64_t ldo, int lsb, hipStream_t st) {
+    GETMI_CHECK_ARG(M >= 0 && M <= 16 && N >= 0 && N <= 0x7fff0000 && K > 0 && K <= 0x7fff0000, "linear_fp8_rows: M=%d N=%d K=%d (M <= 16)", M, N, K);
+    if (M == 0 || N == 0) return GETMI_OK;
+    GETMI_CHECK_ARG(x && B && sb && out && (uintptr_t)out % 2 == 0 && (xt == A_F32 || xt == A_BF16), "linear_fp8_rows: null or odd pointer, or type");
+    GETMI_CHECK_ARG(((uintptr_t)B | (uint64_t)ldb) % 16 == 0 && ldb >= 0 && ldx >= 0 && ldo >= N, "linear_fp8_rows: weight rows have to start on 16 bytes, output rows must not overlap");
+    GETMI_CHECK_ARG(((uintptr_t)sb | (unsigned)lsb) % 4 == 0 && lsb >= 0, "linear_fp8_rows: scale rows have to start on 4 bytes");
+    const int Kp = (K + 127) / 128 * 128, gran = granularity(out, N, ldo);
+    Fp8Args p{(const unsigned char*)x, nullptr, (const unsigned char*)B, (const unsigned char*)sb, bias, (bf16_t*)out,
+              (size_t)ldx * (xt == A_F32 ? 4 : 2), (size_t)ldb, (size_t)ldo, 0, lsb, M, N, Kp, K};
+    return xt == A_F32 ? launch_rows<1, 1, A_F32>(p, gran, st) : launch_rows<1, 1, A_BF16>(p, gran, st);
 }

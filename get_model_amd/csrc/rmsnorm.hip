@@ -15,7 +15,7 @@
 // the column sums' second stage.  Odd width, 51456 x 283 fp32: 20 / 35 us.  One row of 768: 2.1 us.  What got it there: the next
 // row's loads in flight while a row is summed (94 -> 80), element-aligned wide accesses instead of single ones for odd widths (36 ->
 // 20), nt loads for what the caches cannot hold, 1024 workgroups forward / 512 backward.
-#include "common.h"
+#include "fp8.h"
 
 namespace {
 
@@ -42,20 +42,6 @@ __device__ __forceinline__ unsigned max32(unsigned v) {
     v = max(v, dpp<0x140>(v));
     return max(v, xor16(v));
 }
-
-// biased exponent of the smallest power of two 2^e with |amax| <= 448 * 2^e (448 = 1.75 * 2^8); 127 (scale 1) for an all-zero
-// block and for one that holds an infinity or a NaN, which has no scale: its 128 values all become NaN.
-__device__ __forceinline__ unsigned scale_byte(unsigned amax) {
-    const int b = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return (amax == 0u || amax >= 0x7f800000u) ? 127u : (unsigned)max(b, 1);
-}
-__device__ __forceinline__ float inv_scale(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
-__device__ __forceinline__ unsigned pack4fp8(float a, float b, float c, float d, float inv, bool finite) {
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-    v = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, v, true);
-    return finite ? (unsigned)v : 0x7f7f7f7fu;
-}
-__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 template <int T> struct Elem { typedef float type; };
 template <> struct Elem<BF16> { typedef bf16_t type; };

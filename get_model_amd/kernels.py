@@ -559,6 +559,26 @@ def gemm_fp8(a, a_scale, b, b_scale, bias=None):
     return out
 
 
+def linear_rows_fp8(x, b, b_scale, bias=None):
+    """gemm_fp8 of up to 16 rows x[M,K] in fp32 / bf16, quantised inside the product (bit for bit quant_rows_fp8 + gemm_fp8)."""
+    ldx = _rows(x, "x")
+    M, Kd = x.shape
+    N = b.shape[0]
+    if x.dtype not in _TYPE or not 0 < Kd <= 16384 or M > 16:
+        _refuse(f"float32 or bfloat16 of at most 16 rows and 16384 columns is wanted, got {x.dtype} [{M}, {Kd}]")
+    ldb, lsb = _fp8_operand(b, b_scale, -(-N // FP8_BLOCK), "b")
+    if b.shape[1] != -(-Kd // FP8_BLOCK) * FP8_BLOCK:
+        _refuse(f"x {tuple(x.shape)} and b {tuple(b.shape)} do not match")
+    if bias is not None and (bias.dtype != F32 or bias.shape != (N,) or not bias.is_contiguous()):
+        _refuse(f"bias has to be contiguous float32 [{N}]")
+    dev = _on_gpu(x, b, b_scale, bias)
+    out = torch.empty(M, N, dtype=BF16, device=dev)
+    if M and N:
+        lib.launch("getmi_linear_fp8_rows", dev, x.data_ptr(), _TYPE[x.dtype], ldx, b.data_ptr(), b_scale.data_ptr(),
+                   None if bias is None else bias.data_ptr(), out.data_ptr(), M, N, Kd, ldb, N, lsb)
+    return out
+
+
 def _overlaps(t):
     """May two elements of t share memory?  (Dimensions in order of stride: each has to step over all the smaller ones.)"""
     end = 1

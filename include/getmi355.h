@@ -210,6 +210,10 @@ int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb,
                    int64_t lda, int64_t ldb, int64_t ldo, int lsa, int lsb, void* workspace, size_t workspace_bytes, void* stream);
 /* 0 unless the depth is split (few rows, K >= 6144): fp32 partial sums, joined in a fixed order. */
 size_t getmi_gemm_fp8_workspace_bytes(int M, int N, int K);
+/* The same for up to 16 rows that are still in fp32 / bf16 (x[M, K], rows ldx elements apart): quantised inside the product, in one
+ * launch, to the very values getmi_rmsnorm_fp8 without a norm gives.  B[N, K rounded up to 128]. */
+int getmi_linear_fp8_rows(const void* x, int x_type, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M,
+                          int N, int K, int64_t ldb, int64_t ldo, int lsb, void* stream);
 
 /* ---- rotary positions on queries and keys.  No counterpart in the reference (its encoder has no positions). --------------- */
 /* q[B, T, hq, D] -> qo and k[B, T, hk, D] -> ko in one launch (hk may be 0); `strides` is a HOST array of 12 element strides:

@@ -66,6 +66,10 @@ def scales(rows, kb, pitch=None):
     lambda: K.gemm_fp8(fp8(4, 136)[:, :128], scales(4, 1), fp8(8, 128), scales(1, 1)),     # rows off 16 bytes
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1), fp8(8, 128), scales(1, 1), bias=z(7)),
     lambda: K.gemm_fp8(fp8(4, 128), scales(4, 1), fp8(8, 128), scales(1, 1), bias=z(8, dtype=BF16)),
+    lambda: K.linear_rows_fp8(z(17, 100), fp8(8, 128), scales(1, 1)),                  # too many rows
+    lambda: K.linear_rows_fp8(z(4, 200), fp8(8, 128), scales(1, 1)),                   # deeper than the weight
+    lambda: K.linear_rows_fp8(z(4, 100, dtype=torch.float16), fp8(8, 128), scales(1, 1)),
+    lambda: K.linear_rows_fp8(z(4, 100), fp8(8, 128), scales(1, 1), bias=z(7)),
 ])
 def test_products_refuse(call):
     with pytest.raises(ValueError):
@@ -157,6 +161,9 @@ def test_c_entries_check_before_they_launch():
         ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 3, 4, 4, n, 0, n)),       # output rows overlap
         ("getmi_gemm_fp8", (p, p, p, p, n, p, 4, 4, 128, 128, 128, 4, 5, 4, n, 0, n)),       # scale rows off 4 bytes
         ("getmi_gemm_fp8", (p, p, p, p, n, p, 64, 64, 8192, 8192, 8192, 64, 64, 64, n, 0, n)),     # split depth without workspace
+        ("getmi_linear_fp8_rows", (p, 0, 128, p, p, n, p, 17, 64, 128, 128, 64, 4, n)),            # too many rows
+        ("getmi_linear_fp8_rows", (p, 2, 128, p, p, n, p, 4, 64, 128, 128, 64, 4, n)),             # unknown type
+        ("getmi_linear_fp8_rows", (p, 0, 128, p, p, n, p, 4, 64, 128, 100, 64, 4, n)),             # rows off 16 bytes
         ("getmi_rotary", (p, p, 1, n, n, 0, n, 0, 1, 1, 8, 8, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),      # no strides
         ("getmi_rotary", (p, p, 1, n, n, 0, p, 0, 1, 1, 8, 7, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),      # odd columns
         ("getmi_rotary", (p, p, 1, n, n, 0, p, 0, 1, 1, 8, 16, p, n, 0, 0, 0, 0, 0, 0, 1.0, n)),     # more than the head has

@@ -326,6 +326,24 @@ def test_gemm_fp8_strided_rows_nan_rows_and_no_rows():
     assert K.gemm_fp8(*qa, qb[0][:0], qb[1][:0]).shape == (M, 0)
 
 
+@pytest.mark.parametrize("M,N,Kd", [(1, 1, 1), (1, 768, 768), (3, 130, 283), (16, 2304, 768), (9, 8200, 1000), (16, 64, 16384), (2, 33, 129), (5, 40, 8191)])
+@pytest.mark.parametrize("xt", [BF16, F32])
+def test_linear_of_few_rows_is_quantisation_and_product(M, N, Kd, xt):
+    wide = rnd(M, Kd + 5, seed=1, dtype=xt) * torch.exp(2 * rnd(M, 1, seed=2)).to(xt)
+    wide[0, :min(Kd, 128)] = 0
+    qb, bias = K.quant_blocks_fp8(rnd(N, Kd, seed=3, scale=0.1)), rnd(N, seed=4)
+    for x in (wide[:, :Kd], wide[:, 3:3 + Kd], wide[:, :Kd].contiguous(), wide[:1, :Kd].expand(M, Kd)):
+        want = K.gemm_fp8(*K.quant_rows_fp8(x), *qb, bias)
+        assert torch.equal(K.linear_rows_fp8(x, *qb, bias), want)
+    if M > 1:
+        bad = wide[:, :Kd].clone()
+        bad[1, Kd - 1] = float("inf")
+        got = K.linear_rows_fp8(bad, *qb)
+        keep = torch.arange(M, device="cuda") != 1
+        assert got[1].isnan().all() and torch.equal(got[keep], K.linear_rows_fp8(wide[:, :Kd], *qb)[keep])
+    assert K.linear_rows_fp8(wide[:0, :Kd], *qb).shape == (0, N)
+
+
 def test_linear_fp8_and_its_weight_copy():
     x, w = rnd(2, 5, 300, seed=1, dtype=BF16), torch.nn.Parameter(rnd(140, 300, seed=2, scale=0.1))
     b = rnd(140, seed=3)
