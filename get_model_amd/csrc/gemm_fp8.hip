@@ -627,20 +627,6 @@ template <int RB, int GR> static int launch_256p(const Fp8Args& p, hipStream_t s
     GETMI_CHECK_LAUNCH("gemm_fp8");
     return GETMI_OK;
 }
-// Relative time of one round of tiles of 256 / 224 / 192 rows on all CUs.
-static double round_time(int rb) { return rb == 4 ? 1.0 : rb == 3 ? 0.93 : 0.87; }
-template <int GR> static int launch_big(const Fp8Args& p, hipStream_t st) {
-    const int cus = getmi_cu_budget(), tn = (p.N + 255) / 256;
-    int best = 4;
-    double cost = 0;
-    for (int rb = 4; rb >= 2; --rb) {
-        const int bm = 128 + 32 * rb, tiles = ((p.M + bm - 1) / bm) * tn;
-        const double c = (double)((tiles + cus - 1) / cus) * round_time(rb);
-        if (cost == 0 || c < cost - 1e-9) { cost = c; best = rb; }
-    }
-    return best == 4 ? launch_256p<4, GR>(p, st) : best == 3 ? launch_256p<3, GR>(p, st) : launch_256p<2, GR>(p, st);
-}
-
 template <int MT, int NT, int AT = A_FP8> static int launch_rows(const Fp8Args& p, int gran, hipStream_t st) {
     const int nkb = p.K / 128, wgs = ((p.N + 16 * NT - 1) / (16 * NT)) * ((p.M + 16 * MT - 1) / (16 * MT));
     const int W = nkb >= 32 && wgs <= 256 ? 16 : nkb >= 16 ? 8 : 4;      // 4, 8 and 16 measure alike where either applies
@@ -661,6 +647,44 @@ static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStr
     return GETMI_OK;
 }
 
+// What a launch takes, in us (see plan_of): 64 x 64 tiles; a round of 256 / 224 / 192-row tiles on the part `fill` of the CUs.
+static double tile_time(int M, int N, int nk) {
+    const double t = (double)((M + 63) / 64) * ((N + 63) / 64) * 1.1e-3;
+    return 2.5 + nk * (t > 0.34 ? t : 0.34);
+}
+static double round_time(int rb, int nk, double fill) {
+    return (nk * (1.15 + 0.7 * fill) + 3.5) * (rb == 4 ? 1.0 : rb == 3 ? 0.93 : 0.87);
+}
+
+template <int GR> static int launch_256p(const Fp8Args& p, int rb, hipStream_t st) {
+    return rb == 4 ? launch_256p<4, GR>(p, st) : rb == 3 ? launch_256p<3, GR>(p, st) : launch_256p<2, GR>(p, st);
+}
+// Tile height: the one whose rounds take least.  Where the last round would hold very few tiles, whole rounds only, and the rows
+// behind them go to 64 x 64 tiles in a second launch (charged twice: alone on the chip they run at half their rate).  51456 x 2304 x
+// 768, 7.07 rounds: 113 -> 109 us; 33000 x 512 x 4096, 1.01 rounds: 90 -> 74; at 2.25 rounds of 6000^3 it would cost 195 -> 218.
+template <int GR> static int launch_big(const Fp8Args& p, int gran, hipStream_t st) {
+    const int cus = getmi_cu_budget(), tn = (p.N + 255) / 256, nk = p.K >> 7;
+    int best = 4, rows = p.M;
+    double cost = 0;
+    for (int rb = 4; rb >= 2; --rb) {
+        const int bm = 128 + 32 * rb;
+        const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * tn, before = (tiles - 1) / cus;      // whole rounds before the last
+        const double most = before * round_time(rb, nk, 1.0), whole = most + round_time(rb, nk, (double)(tiles - before * cus) / cus);
+        if (cost == 0 || whole < cost - 1e-9) { cost = whole; best = rb; rows = p.M; }
+        const int64_t cut = before * cus / tn * bm;
+        if (cut > 0 && cut < p.M) {
+            const double c = most + 2.0 * tile_time((int)(p.M - cut), p.N, nk);
+            if (c < cost - 1e-9) { cost = c; best = rb; rows = (int)cut; }
+        }
+    }
+    Fp8Args q = p;
+    q.M = rows;
+    if (const int rc = launch_256p<GR>(q, best, st)) return rc;
+    if (rows == p.M) return GETMI_OK;
+    q.A += (size_t)rows * p.lda; q.sa += (size_t)rows * p.lsa; q.out += (size_t)rows * p.ldo; q.M = p.M - rows;
+    return launch_tile(q, gran, 1, nullptr, st);
+}
+
 // Which kernel takes a product: by its shape alone.  Both sides measured on MI355X (us, back to back, operands in rotation):
 //   up to 16 rows    rows kernel: 1 x 8192 x 8192 13.6 (4.9 TB/s) against 64-row tiles 22.5; 8 x 768 x 8192 9.0 against 21.7.  Two
 //                    16-row groups of B a workgroup where both sides are wide (16 x 8192 x 8192 20.0 -> 17.2; 1 row: 13.6 -> 16.6)
@@ -677,7 +701,7 @@ static Plan plan_of(int M, int N, int K) {
     if (M <= 32 && N <= 4096) return Plan{ROWS21, 1};
     const int nk = K >> 7;
     const double t64 = (double)((M + 63) / 64) * ((N + 63) / 64), t256 = (double)((M + 255) / 256) * ((N + 255) / 256);
-    const double small = 2.5 + nk * (t64 * 1.1e-3 > 0.34 ? t64 * 1.1e-3 : 0.34);
+    const double small = tile_time(M, N, nk);
     const double rounds = (double)(((int64_t)t256 + 255) / 256);
     const double large = 2.0 + rounds * (nk * (1.15 + 0.7 * (t256 < 256 ? t256 / 256 : 1.0)) + 3.5);
     if (nk >= 2 && large < small) return Plan{BIG, 1};
@@ -714,7 +738,7 @@ int getmi_gemm_fp8_impl(const void* A, const void* sa, const void* B, const void
     if (pl.kind == ROWS11) return launch_rows<1, 1>(p, gran, st);
     if (pl.kind == ROWS12) return launch_rows<1, 2>(p, gran, st);
     if (pl.kind == ROWS21) return launch_rows<2, 1>(p, gran, st);
-    if (pl.kind == BIG && fits) return gran == 8 ? launch_big<8>(p, st) : gran >= 2 ? launch_big<2>(p, st) : launch_big<1>(p, st);
+    if (pl.kind == BIG && fits) return gran == 8 ? launch_big<8>(p, gran, st) : gran >= 2 ? launch_big<2>(p, gran, st) : launch_big<1>(p, gran, st);
     return launch_tile(p, gran, pl.splits, (float*)workspace, st);
 }
 

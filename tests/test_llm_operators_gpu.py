@@ -276,7 +276,9 @@ SHAPES = [(1, 1, 1), (1, 17, 128), (1, 768, 768), (1, 2304, 300), (2, 130, 1000)
           (13000, 1026, 300), (26000, 513, 384),
           # the depth split in two and in four, and the shapes next to those; two row groups of either operand
           (64, 300, 8192), (100, 767, 8200), (40, 8192, 6144), (33, 5001, 6272), (64, 2048, 6016), (12, 8200, 1024), (9, 8193, 300),
-          (32, 4096, 700), (20, 33, 9000), (31, 8192, 256)]
+          (32, 4096, 700), (20, 33, 9000), (31, 8192, 256),
+          # just over a round of large tiles: the last rows go to small ones
+          (33000, 512, 1024), (32900, 511, 1100), (57600, 300, 1000)]
 
 
 @pytest.mark.parametrize("M,N,Kd", SHAPES)
