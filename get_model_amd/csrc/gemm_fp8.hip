@@ -287,7 +287,11 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Fp8Args p, int gran,
 // K-tile in and the tile out, at 16 - 20 bytes a clock (counters: matrix units 65 % busy at 8192^3, LDS 26 %, bank conflicts 2 %):
 // 51456 x 2304 x 768 carries 948 MB over it.  Tried without gain: wave priorities around the matrix instructions, reads before the
 // next half-tile's issue, two launches of different tile height against the partial last round, other tile orders, a K order turned
-// per XCD; output stores through the cache instead of past it: 110 -> 116 us.
+// per XCD; a strip of B resident in LDS with rows of A streamed past it (115 us against 112, with a quarter less operand traffic).
+// The output costs 16 - 24 of the 100 us at 51456 x 2304 (without its stores K = 256 / 768 / 1536 take 47 / 90 / 160 us, with them 71 /
+// 106 / 179, and the same when they all go to 4 MB, so memory is not it: the CU's path again, a fill of that size takes 30).  They leave
+// as whole 128-byte lines through LDS, past the cache: through it 110 -> 116; exchanged between lanes by v_permlane16_swap instead,
+// in half lines, 100 -> 116.
 // ------------------------------------------------------------------------------------------------
 #define F8_SCALES 131072
 #define F8_BIAS (F8_SCALES + 2 * 2048)
