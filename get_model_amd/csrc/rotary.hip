@@ -22,7 +22,7 @@ struct Args {
     Side q, k;
     const void* pos; const double* inv_freq;
     int64_t pb, pt, offset;
-    int T, ntok, D, R, tb, pos64, copy;
+    int T, ntok, D, R, tb, pos64, copy, first;
     float magnitude, sign;
 };
 
@@ -96,7 +96,7 @@ template <int T, bool HALF, int V, bool NT>
 __global__ __launch_bounds__(256) void rotary_kernel(Args p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr bool TWO = HALF || V == 1;
-    const int half = p.R >> 1, tok0 = blockIdx.x * p.tb, tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+    const int half = p.R >> 1, tok0 = p.first + blockIdx.x * p.tb, tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
     const int tokens = min(p.tb, p.ntok - tok0);
     int64_t* base = reinterpret_cast<int64_t*>(smem);                      // [tb][4]: where the token starts in q, qo, k, ko
     float2* table = reinterpret_cast<float2*>(smem + p.tb * 32);           // [tb][R/2]
@@ -205,8 +205,14 @@ template <int T, bool HALF, int V> void launch(Args& a, hipStream_t st) {
     // 32768 x 18 x 128 fp32 126 -> 115 us, interleaved bf16 58 -> 55).  Halves of 64 bytes share lines and lose: 63 -> 65.
     const size_t size = T == F32 ? 4 : 2;
     const bool nt = V > 1 && 2 * size * a.ntok * heads * a.D > ((size_t)256 << 20) && (!HALF || half * size % 128 == 0);
-    if (nt) hipLaunchKernelGGL((rotary_kernel<T, HALF, V, (V > 1)>), dim3(blocks, gy), dim3(bx, by), lds, st, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, HALF, V, false>), dim3(blocks, gy), dim3(bx, by), lds, st, a);
+    // (a launch is at most 2^32 - 1 threads wide)
+    const int most = 1 << 23;
+    for (int b0 = 0; b0 < blocks; b0 += most) {
+        const dim3 grid(blocks - b0 < most ? blocks - b0 : most, gy);
+        a.first = b0 * a.tb;
+        if (nt) hipLaunchKernelGGL((rotary_kernel<T, HALF, V, (V > 1)>), grid, dim3(bx, by), lds, st, a);
+        else hipLaunchKernelGGL((rotary_kernel<T, HALF, V, false>), grid, dim3(bx, by), lds, st, a);
+    }
 }
 
 }  // namespace

@@ -914,8 +914,8 @@ def _make_w_fp8(t):
 
 
 def w_fp8(w):
-    """The (q, scale) pair of a weight [N, K], kept like the bf16 copies and made anew when the parameter changes.  A copy made
-    inside a graph capture belongs to that graph and is not kept."""
+    """The (q, scale) pair of a weight [N, K], kept like the bf16 copies and made anew when the parameter changes (code that writes
+    `param.data` by hand calls WEIGHTS.clear()).  A copy made inside a graph capture belongs to that graph and is not kept."""
     _need_gpu(w)
     if torch.cuda.is_current_stream_capturing():
         hit = WEIGHTS.current(w, "fp8")
@@ -934,7 +934,7 @@ def linear_fp8(x, weight, bias=None):
     """x @ weight^T + bias in 8-bit floating point (e4m3, one power-of-two scale per 128 columns of a row of x and per 128 x 128
     block of the weight), fp32 accumulation, bf16 out.  Inference only.
 
-    x: [..., K] fp32 / bf16, quantised here, or the (q, scale) pair of rms_norm_fp8 / kernels.quant_rows_fp8 (result [M, N]).
+    x: [..., K] fp32 / bf16 (K <= 16384), quantised here, or the (q, scale) pair of rms_norm_fp8 / kernels.quant_rows_fp8 (result [M, N]).
     weight: [N, K] fp32 / bf16 (a Parameter's 8-bit copy is kept, see w_fp8), or the pair of kernels.quant_blocks_fp8.
     bias: fp32 [N]."""
     pair, wpair = isinstance(x, (tuple, list)), isinstance(weight, (tuple, list))

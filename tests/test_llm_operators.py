@@ -177,6 +177,14 @@ def test_c_entries_check_before_they_launch():
     assert h.getmi_rotary(n, n, 0, n, n, 0, n, 0, 1, 1, 8, 8, n, n, 0, 0, 0, 0, 0, 0, 1.0, n) == 0
 
 
+def test_c_entries_refuse_more_than_a_launch_holds():
+    h, p, n, most = lib.load(), 4096, None, 0x7fff0000
+    assert h.getmi_gemm_fp8(p, p, p, p, n, p, most, 64, 128, 128, 128, 64, 4, 4, n, 0, n) == 1
+    assert b"too large" in h.getmi_last_error()
+    assert h.getmi_linear_fp8_rows(p, 0, 128, p, p, n, p, 4, most, 128, 128, most, 4, n) == 1
+    assert b"too large" in h.getmi_last_error()
+
+
 def test_rotary_frequencies():
     c, base = 64, 10000.0
     plain, m = Fn.rotary_frequencies(c, base)

@@ -511,6 +511,30 @@ def test_rows_past_four_gigabytes():
     assert torch.equal(tf, want)
 
 
+def test_a_product_whose_output_passes_four_gigabytes():
+    """Rows past the large kernel's 32-bit reach go in launches of their own (small integers: every order of the sums is exact)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    M, N, Kp = 950001, 2304, 256
+    ints = [torch.randint(-2, 3, (n, Kp), generator=g, device="cuda", dtype=torch.int8).to(F32).to(K.FP8) for n in (M, N)]
+    sa, sb = (torch.full((n, 4), 127, dtype=torch.uint8, device="cuda").view(K.SCALE)[:, :2] for n in (M, N // 128))
+    out = K.gemm_fp8(ints[0], sa, ints[1], sb)
+    assert out.numel() * 2 > 1 << 32
+    w = ints[1].float().t().contiguous()
+    for r in (0, 474500, 475136, 949000):
+        assert torch.equal(out[r:r + 1001], (ints[0][r:r + 1001].float() @ w).to(BF16)), r
+    for r in range(0, M, 100000):      # every row against calls that one launch covers
+        assert torch.equal(out[r:r + 100000], K.gemm_fp8(ints[0][r:r + 100000], sa[r:r + 100000], ints[1], sb)), r
+
+
+def test_rotary_of_more_tokens_than_one_launch_takes():
+    T, D = (1 << 23) + 700, 512
+    q = rnd(1, 1, 1, D, dtype=BF16).expand(1, T, 1, D)
+    inv, _ = Fn.rotary_frequencies(D, device="cuda")
+    out = Fn.rotary(q, None, inv)
+    for t in (0, 4096, (1 << 23) - 200, T - 300):
+        assert torch.equal(out[:, t:t + 300], Fn.rotary(q[:, :300], None, inv, offset=t)), t
+
+
 # ----------------------------------------------------------------------------------------------------- together, and around
 def test_the_chain_into_attention():
     """Norm with residual -> 8-bit projection -> rotary in place on the packed queries and keys -> the framework's attention."""
