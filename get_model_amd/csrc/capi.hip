@@ -75,6 +75,8 @@ int getmi_gemm_fp8_impl(const void*, const void*, const void*, const void*, cons
 size_t getmi_gemm_fp8_workspace_bytes_impl(int M, int N, int K);
 int getmi_linear_fp8_rows_impl(const void*, int, int64_t, const void*, const void*, const float*, void*, int, int, int, int64_t, int64_t, int,
                                hipStream_t);
+int getmi_linear_fp8_tiles_impl(const void*, int, int64_t, const void*, const void*, const float*, void*, int, int, int, int64_t, int64_t, int,
+                                hipStream_t);
 int getmi_rotary_impl(const void*, void*, int, const void*, void*, int, const int64_t*, int, int, int, int, int, const double*, const void*,
                       int, int64_t, int64_t, int64_t, int, int, float, hipStream_t);
 
@@ -260,6 +262,10 @@ int getmi_gemm_fp8(const void* A, const void* sa, const void* B, const void* sb,
 int getmi_linear_fp8_rows(const void* x, int x_type, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M, int N,
                           int K, int64_t ldb, int64_t ldo, int lsb, void* stream) {
     return getmi_linear_fp8_rows_impl(x, x_type, ldx, B, sb, bias, out, M, N, K, ldb, ldo, lsb, ST(stream));
+}
+int getmi_linear_fp8_tiles(const void* x, int x_type, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M, int N,
+                           int K, int64_t ldb, int64_t ldo, int lsb, void* stream) {
+    return getmi_linear_fp8_tiles_impl(x, x_type, ldx, B, sb, bias, out, M, N, K, ldb, ldo, lsb, ST(stream));
 }
 size_t getmi_gemm_fp8_workspace_bytes(int M, int N, int K) { return getmi_gemm_fp8_workspace_bytes_impl(M, N, K); }
 int getmi_rotary(const void* q, void* qo, int hq, const void* k, void* ko, int hk, const int64_t* strides, int type, int B, int T, int D,

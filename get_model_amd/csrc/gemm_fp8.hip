@@ -188,10 +188,51 @@ template <int N> __device__ __forceinline__ void wait_vm() {
 // the CU's path to the caches (16 KiB a K-tile at about 24 bytes a clock), not the depth of the ring: rings of 2, 4 and 6 and tiles
 // of 128 x 64, 64 x 128, 128 x 128, 64 x 32, 32 x 64 and 32 x 32 measured within 10 % or slower over 28 shapes (4020 x 768 x 768:
 // 8.6 us host-bound, 1000 x 2304 x 2304: 15.4).  splits > 1: workgroup (tile, s) takes the s-th part of the depth.
+//
+// AT: e4m3 rows, or 16- / 32-bit rows (p.sa unused, p.lda in bytes, p.Ka columns) that are quantised on their way into LDS: four
+// threads a row, their pieces of 8 columns side by side, loaded a K-tile ahead; two slots of A's image and scales behind B's ring.
+// A K-tile takes 0.87 us there (the load's latency shows) or 2.4 ns x tiles.  Loads two K-tiles ahead measured the same: hipcc cannot
+// count loads that a branch may skip and waits for all of them.
 // ------------------------------------------------------------------------------------------------
-constexpr int T64_SLOTS = 3, T64_STAGE = 128 * 128 + 1024, T64_OPS = 5;      // LDS-DMA operations a wave and K-tile
+template <int AT> struct Tile64 {
+    static constexpr bool Q = AT != A_FP8;
+    static constexpr int SLOTS = 3, IMAGE = (Q ? 64 : 128) * 128, STAGE = IMAGE + 1024, OPS = Q ? 3 : 5;      // LDS-DMA operations a wave and K-tile
+    static constexpr int A_SLOT = 64 * 128 + 256, LDS = SLOTS * STAGE + (Q ? 2 * A_SLOT : 0);
+};
+// eight consecutive columns of a 16- or 32-bit row as they lie in memory, of which n exist (the others are zero)
+template <int AT> struct Eight;
+template <> struct Eight<A_BF16> {
+    typedef __attribute__((ext_vector_type(8), aligned(2))) unsigned short V;
+    V v;
+    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
+        const bf16_t* p = reinterpret_cast<const bf16_t*>(row) + col;
+        v = V{0, 0, 0, 0, 0, 0, 0, 0};
+        if (n >= 8) v = *reinterpret_cast<const V*>(p);
+        else if (n > 0)      // (all loads, then the choice: a load under a condition of its own would wait for the one before)
+#pragma unroll
+            for (int i = 0; i < 7; ++i) { const unsigned short e = p[min(i, n - 1)]; v[i] = i < n ? e : 0; }
+    }
+    __device__ __forceinline__ float at(int i) const { return bf2f(v[i]); }
+};
+template <> struct Eight<A_F32> {
+    typedef __attribute__((ext_vector_type(4), aligned(4))) float V;
+    V v[2];
+    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
+        const float* p = reinterpret_cast<const float*>(row) + col;
+        v[0] = v[1] = V{0.f, 0.f, 0.f, 0.f};
+        if (n >= 8) { v[0] = *reinterpret_cast<const V*>(p); v[1] = *reinterpret_cast<const V*>(p + 4); }
+        else if (n > 0)
+#pragma unroll
+            for (int i = 0; i < 7; ++i) { const float e = p[min(i, n - 1)]; v[i >> 2][i & 3] = i < n ? e : 0.f; }
+    }
+    __device__ __forceinline__ float at(int i) const { return v[i >> 2][i & 3]; }
+};
+template <> struct Eight<A_FP8> {};
 
+template <int AT>
 __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws) {
+    typedef Tile64<AT> T;
+    constexpr bool Q = T::Q;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1, nkb = p.K >> 7;
@@ -205,12 +246,50 @@ __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran,
         const int row = (i * 4 + wave) * 8 + (lane >> 3), chunk = ((lane & 7) ^ ((row >> 1) & 7)) << 4;
         src[i] = (row < 64 ? p.A + (size_t)min(m0 + row, p.M - 1) * p.lda : p.B + (size_t)min(n0 + row - 64, p.N - 1) * p.ldb) + chunk;
     }
-    const unsigned char* ssrc = tid < 64 ? p.sa + (size_t)min(m0 + tid, p.M - 1) * p.lsa : p.sb + (size_t)(n0 >> 7) * p.lsb;
+    const unsigned char* ssrc = !Q && tid < 64 ? p.sa + (size_t)min(m0 + tid, p.M - 1) * p.lsa : p.sb + (size_t)(n0 >> 7) * p.lsb;
     auto issue = [&](int k, int slot) {
-        char* b = smem + slot * T64_STAGE;
+        char* b = smem + slot * T::STAGE;
+        constexpr int I0 = Q ? 2 : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) glds16(src[i] + (size_t)(kb0 + k) * 128, b + (i * 4 + wave) * 1024);
-        glds4(ssrc + ((kb0 + k) & ~3), b + 128 * 128 + wave * 256);
+        for (int i = I0; i < 4; ++i) glds16(src[i] + (size_t)(kb0 + k) * 128, b + ((i - I0) * 4 + wave) * 1024);
+        glds4(ssrc + ((kb0 + k) & ~3), b + T::IMAGE + wave * 256);
+    };
+    const int qrow = tid >> 2, qpiece = tid & 3;
+    const unsigned char* arow = p.A + (size_t)min(m0 + qrow, p.M - 1) * p.lda;
+    Eight<AT> raw[4];
+    auto load_a = [&](int k) {
+        if constexpr (Q) {
+            const int col = (kb0 + k) * 128 + qpiece * 8;
+            if ((kb0 + k) * 128 + 128 <= p.Ka) {      // (the same for all: no branch per piece but in the last block)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[i].load(arow, col + i * 32, 8);
+            } else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[i].load(arow, col + i * 32, p.Ka - col - i * 32);
+        }
+    };
+    auto quantise_a = [&](int k) {
+        if constexpr (Q) {
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max(m, abs_bits(raw[i].at(j)));
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true));      // lanes 1 and 2 apart: the row's four
+            m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, true));
+            const unsigned byte = scale_byte(m), slot = lds_addr(smem) + T::SLOTS * T::STAGE + (k & 1) * T::A_SLOT;
+            const float inv = inv_scale(byte);
+            const bool finite = m < 0x7f800000u;
+            // (inline asm: before a write it can see hipcc may wait for the LDS-DMA in flight)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int piece = i * 4 + qpiece;
+                const u32x2 v = {pack4fp8(raw[i].at(0), raw[i].at(1), raw[i].at(2), raw[i].at(3), inv, finite),
+                                 pack4fp8(raw[i].at(4), raw[i].at(5), raw[i].at(6), raw[i].at(7), inv, finite)};
+                asm volatile("ds_write_b64 %0, %1" ::"v"(slot + qrow * 128 + (((piece >> 1) ^ ((qrow >> 1) & 7)) << 4) + (piece & 1) * 8), "v"(v) : "memory");
+            }
+            if (qpiece == 0) asm volatile("ds_write_b32 %0, %1" ::"v"(slot + 64 * 128 + qrow * 4), "v"(byte) : "memory");
+        }
     };
     f32x4 acc[2][2];
 #pragma unroll
@@ -219,14 +298,25 @@ __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran,
         for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int fsw = (r >> 1) & 7;
     const unsigned lds0 = lds_addr(smem), off0 = r * 128 + ((c ^ fsw) << 4), off1 = r * 128 + (((4 + c) ^ fsw) << 4);
+    load_a(0);
     issue(0, 0);
-    if (nk > 1) issue(1, 1);
+    quantise_a(0);
+    if (nk > 1) {
+        load_a(1);
+        issue(1, 1);
+    }
     int slot = 0;
     for (int k = 0; k < nk; ++k) {
-        if (k + 1 < nk) wait_vm<T64_OPS>(); else wait_vm<0>();      // K-tile k has landed (this wave's share), k + 1 stays in flight
-        phase_barrier();                                              // ... every wave's share; and K-tile k - 1 has been read by all
-        if (k + 2 < nk) issue(k + 2, slot == 0 ? 2 : slot - 1);
-        const unsigned b = lds0 + slot * T64_STAGE, ab = b + wm * 4096, bb = b + 8192 + wn * 4096, sc = b + 128 * 128;
+        if (k + 1 < nk) wait_vm<T::OPS>(); else wait_vm<0>();      // K-tile k has landed (this wave's share), k + 1 stays in flight
+        if constexpr (Q) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        phase_barrier();                                             // ... every wave's share; and K-tile k - 1 has been read by all
+        if (k + 1 < nk) quantise_a(k + 1);
+        if (k + 2 < nk) {
+            load_a(k + 2);
+            issue(k + 2, slot == 0 ? 2 : slot - 1);
+        }
+        const unsigned b = lds0 + slot * T::STAGE, as = Q ? lds0 + T::SLOTS * T::STAGE + (k & 1) * T::A_SLOT : b;
+        const unsigned ab = as + wm * 4096, bb = b + (Q ? 0 : 8192) + wn * 4096, sc = b + T::IMAGE, asc = Q ? as + 64 * 128 : sc;
         const unsigned a0 = ab + off0, a1 = ab + off1, b0 = bb + off0, b1 = bb + off1;
         u32x4 fa[2][2], fb[2][2];
         unsigned sa[2], sb;
@@ -238,14 +328,14 @@ __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran,
             "s_waitcnt lgkmcnt(0)"
             : "=&v"(sb), "=&v"(sa[0]), "=&v"(sa[1]), "=&v"(fa[0][0]), "=&v"(fa[0][1]), "=&v"(fa[1][0]), "=&v"(fa[1][1]), "=&v"(fb[0][0]),
               "=&v"(fb[0][1]), "=&v"(fb[1][0]), "=&v"(fb[1][1])
-            : "v"(sc), "v"(sc + (wm * 32 + r) * 4), "v"(a0), "v"(a1), "v"(b0), "v"(b1)
+            : "v"(sc), "v"(asc + (wm * 32 + r) * 4), "v"(a0), "v"(a1), "v"(b0), "v"(b1)
             : "memory");
-        const int sh = ((kb0 + k) & 3) * 8;
+        const int sh = ((kb0 + k) & 3) * 8, sha = Q ? 0 : sh;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                acc[i][j] = mfma_fp8(join8(fb[j][0], fb[j][1]), join8(fa[i][0], fa[i][1]), acc[i][j], (int)(sb >> sh), (int)(sa[i] >> sh));
+                acc[i][j] = mfma_fp8(join8(fb[j][0], fb[j][1]), join8(fa[i][0], fa[i][1]), acc[i][j], (int)(sb >> sh), (int)(sa[i] >> sha));
         slot = slot == 2 ? 0 : slot + 1;
     }
 #pragma unroll
@@ -641,10 +731,10 @@ template <int MT, int NT, int AT = A_FP8> static int launch_rows(const Fp8Args& 
     GETMI_CHECK_LAUNCH("gemm_fp8");
     return GETMI_OK;
 }
-static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStream_t st) {
+template <int AT = A_FP8> static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStream_t st) {
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
     GETMI_CHECK_ARG(tiles * splits < 1 << 24, "gemm_fp8: M=%d N=%d too large", p.M, p.N);      // a launch is at most 2^32 - 1 threads wide
-    hipLaunchKernelGGL(gemm_fp8_tile_kernel, dim3((unsigned)(tiles * splits)), dim3(256), T64_SLOTS * T64_STAGE, st, p, gran, splits, ws);
+    hipLaunchKernelGGL(gemm_fp8_tile_kernel<AT>, dim3((unsigned)(tiles * splits)), dim3(256), Tile64<AT>::LDS, st, p, gran, splits, ws);
     if (splits > 1) {
         const int64_t blocks = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
         hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p, gran, splits,
@@ -772,4 +862,18 @@ int getmi_linear_fp8_rows_impl(const void* x, int xt, int64_t ldx, const void* B
     Fp8Args p{(const unsigned char*)x, nullptr, (const unsigned char*)B, (const unsigned char*)sb, bias, (bf16_t*)out,
               (size_t)ldx * (xt == A_F32 ? 4 : 2), (size_t)ldb, (size_t)ldo, 0, lsb, M, N, Kp, K};
     return xt == A_F32 ? launch_rows<1, 1, A_F32>(p, gran, st) : launch_rows<1, 1, A_BF16>(p, gran, st);
+}
+
+// Any number of rows of fp32 / bf16, quantised inside the product by every 64 x 64 tile that reads them.
+int getmi_linear_fp8_tiles_impl(const void* x, int xt, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M, int N,
+                                int K, int64_t ldb, int64_t ldo, int lsb, hipStream_t st) {
+    GETMI_CHECK_ARG(M >= 0 && M <= 0x7fff0000 && N >= 0 && N <= 0x7fff0000 && K > 0 && K <= 0x7fff0000, "linear_fp8_tiles: M=%d N=%d K=%d", M, N, K);
+    if (M == 0 || N == 0) return GETMI_OK;
+    GETMI_CHECK_ARG(x && B && sb && out && (uintptr_t)out % 2 == 0 && (xt == A_F32 || xt == A_BF16), "linear_fp8_tiles: null or odd pointer, or type");
+    GETMI_CHECK_ARG(((uintptr_t)B | (uint64_t)ldb) % 16 == 0 && ldb >= 0 && ldx >= 0 && ldo >= N, "linear_fp8_tiles: weight rows have to start on 16 bytes, output rows must not overlap");
+    GETMI_CHECK_ARG(((uintptr_t)sb | (unsigned)lsb) % 4 == 0 && lsb >= 0, "linear_fp8_tiles: scale rows have to start on 4 bytes");
+    const int Kp = (K + 127) / 128 * 128, gran = granularity(out, N, ldo);
+    Fp8Args p{(const unsigned char*)x, nullptr, (const unsigned char*)B, (const unsigned char*)sb, bias, (bf16_t*)out,
+              (size_t)ldx * (xt == A_F32 ? 4 : 2), (size_t)ldb, (size_t)ldo, 0, lsb, M, N, Kp, K};
+    return xt == A_F32 ? launch_tile<A_F32>(p, gran, 1, nullptr, st) : launch_tile<A_BF16>(p, gran, 1, nullptr, st);
 }

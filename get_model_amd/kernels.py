@@ -561,11 +561,20 @@ def gemm_fp8(a, a_scale, b, b_scale, bias=None):
 
 def linear_rows_fp8(x, b, b_scale, bias=None):
     """gemm_fp8 of up to 16 rows x[M,K] in fp32 / bf16, quantised inside the product (bit for bit quant_rows_fp8 + gemm_fp8)."""
+    return _linear_inside("getmi_linear_fp8_rows", 16, x, b, b_scale, bias)
+
+
+def linear_tiles_fp8(x, b, b_scale, bias=None):
+    """The same for any number of rows: every 64 x 64 tile quantises the rows it reads, which pays where there are few tiles."""
+    return _linear_inside("getmi_linear_fp8_tiles", _MOST, x, b, b_scale, bias)
+
+
+def _linear_inside(entry, most, x, b, b_scale, bias):
     ldx = _rows(x, "x")
     M, Kd = x.shape
     N = b.shape[0]
-    if x.dtype not in _TYPE or not 0 < Kd <= 16384 or M > 16:
-        _refuse(f"float32 or bfloat16 of at most 16 rows and 16384 columns is wanted, got {x.dtype} [{M}, {Kd}]")
+    if x.dtype not in _TYPE or not 0 < Kd <= 16384 or M > most:
+        _refuse(f"float32 or bfloat16 of at most {most} rows and 16384 columns is wanted, got {x.dtype} [{M}, {Kd}]")
     ldb, lsb = _fp8_operand(b, b_scale, -(-N // FP8_BLOCK), "b")
     if b.shape[1] != -(-Kd // FP8_BLOCK) * FP8_BLOCK:
         _refuse(f"x {tuple(x.shape)} and b {tuple(b.shape)} do not match")
@@ -574,7 +583,7 @@ def linear_rows_fp8(x, b, b_scale, bias=None):
     dev = _on_gpu(x, b, b_scale, bias)
     out = torch.empty(M, N, dtype=BF16, device=dev)
     if M and N:
-        lib.launch("getmi_linear_fp8_rows", dev, x.data_ptr(), _TYPE[x.dtype], ldx, b.data_ptr(), b_scale.data_ptr(),
+        lib.launch(entry, dev, x.data_ptr(), _TYPE[x.dtype], ldx, b.data_ptr(), b_scale.data_ptr(),
                    None if bias is None else bias.data_ptr(), out.data_ptr(), M, N, Kd, ldb, N, lsb)
     return out
 

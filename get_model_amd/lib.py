@@ -62,6 +62,7 @@ _SIGNATURES = {
     "getmi_quant_blocks_fp8": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _i, _vp]),
     "getmi_gemm_fp8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _i, _vp, _sz, _vp]),
     "getmi_linear_fp8_rows": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i, _vp]),
+    "getmi_linear_fp8_tiles": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i, _vp]),
     "getmi_gemm_fp8_workspace_bytes": (_sz, [_i, _i, _i]),
     "getmi_rotary": (_i, [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i64, _i64, _i64, _i, _i, _f, _vp]),
     "getmi_set_cu_limit": (_i, [_i]),

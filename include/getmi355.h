@@ -214,6 +214,9 @@ size_t getmi_gemm_fp8_workspace_bytes(int M, int N, int K);
  * launch, to the very values getmi_rmsnorm_fp8 without a norm gives.  B[N, K rounded up to 128]. */
 int getmi_linear_fp8_rows(const void* x, int x_type, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M,
                           int N, int K, int64_t ldb, int64_t ldo, int lsb, void* stream);
+/* ... and for any number of rows: every 64 x 64 tile quantises the rows it reads (for products of few such tiles). */
+int getmi_linear_fp8_tiles(const void* x, int x_type, int64_t ldx, const void* B, const void* sb, const float* bias, void* out, int M,
+                           int N, int K, int64_t ldb, int64_t ldo, int lsb, void* stream);
 
 /* ---- rotary positions on queries and keys.  No counterpart in the reference (its encoder has no positions). --------------- */
 /* q[B, T, hq, D] -> qo and k[B, T, hk, D] -> ko in one launch (hk may be 0); `strides` is a HOST array of 12 element strides:

@@ -177,6 +177,24 @@ def test_c_entries_check_before_they_launch():
     assert h.getmi_rotary(n, n, 0, n, n, 0, n, 0, 1, 1, 8, 8, n, n, 0, 0, 0, 0, 0, 0, 1.0, n) == 0
 
 
+def test_linear_in_tiles_checks_before_it_launches():
+    h, p, n = lib.load(), 4096, None
+    for args in [(p, 0, 128, p, p, n, p, -1, 64, 128, 128, 64, 4, n),       # rows
+                 (p, 2, 128, p, p, n, p, 17, 64, 128, 128, 64, 4, n),       # unknown type
+                 (p, 0, 128, p, p, n, p, 17, 64, 128, 100, 64, 4, n),       # weight rows off 16 bytes
+                 (p, 0, 128, p, p, n, p, 17, 64, 128, 128, 63, 4, n),       # output rows overlap
+                 (p, 0, 128, p, p, n, p, 17, 64, 128, 128, 64, 5, n),       # scale rows off 4 bytes
+                 (n, 0, 128, p, p, n, p, 17, 64, 128, 128, 64, 4, n)]:      # no x
+        assert h.getmi_linear_fp8_tiles(*args) == 1 and h.getmi_last_error(), args
+    assert h.getmi_linear_fp8_tiles(n, 0, 0, n, n, n, n, 0, 64, 128, 128, 64, 4, n) == 0
+    w = torch.zeros(64, 128).to(K.FP8), torch.zeros(1, 4, dtype=torch.uint8).view(K.SCALE)[:, :1]
+    for x in (torch.zeros(20, 128, dtype=F64), torch.zeros(20, 129), torch.zeros(128), torch.zeros(20, 16385)):
+        with pytest.raises(ValueError):
+            K.linear_tiles_fp8(x, *w)
+    with pytest.raises(RuntimeError):      # no CPU path
+        K.linear_tiles_fp8(torch.zeros(20, 128), *w)
+
+
 def test_c_entries_refuse_more_than_a_launch_holds():
     h, p, n, most = lib.load(), 4096, None, 0x7fff0000
     assert h.getmi_gemm_fp8(p, p, p, p, n, p, most, 64, 128, 128, 128, 64, 4, 4, n, 0, n) == 1

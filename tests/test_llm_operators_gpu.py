@@ -346,6 +346,33 @@ def test_linear_of_few_rows_is_quantisation_and_product(M, N, Kd, xt):
     assert K.linear_rows_fp8(wide[:0, :Kd], *qb).shape == (0, N)
 
 
+@pytest.mark.parametrize("M,N,Kd", [(1, 1, 1), (17, 768, 768), (64, 64, 128), (65, 130, 283), (201, 2304, 768), (100, 33, 1001), (31, 700, 5000), (4020, 256, 768), (70, 70, 9),
+                                    (128, 65, 127), (129, 64, 1028)])
+@pytest.mark.parametrize("xt", [BF16, F32])
+def test_linear_in_tiles_is_quantisation_and_product(M, N, Kd, xt):
+    wide = rnd(M, Kd + 5, seed=1, dtype=xt) * torch.exp(2 * rnd(M, 1, seed=2)).to(xt)
+    wide[0, :min(Kd, 128)] = 0
+    qb, bias = K.quant_blocks_fp8(rnd(N, Kd, seed=3, scale=0.1)), rnd(N, seed=4)
+    for x in (wide[:, :Kd], wide[:, 3:3 + Kd], wide[:, :Kd].contiguous(), wide[:1, :Kd].expand(M, Kd)):
+        assert torch.equal(K.linear_tiles_fp8(x, *qb, bias), K.gemm_fp8(*K.quant_rows_fp8(x), *qb, bias))
+    if M > 1:
+        bad = wide[:, :Kd].clone()
+        bad[1, Kd - 1] = float("inf")
+        got = K.linear_tiles_fp8(bad, *qb)
+        keep = torch.arange(M, device="cuda") != 1
+        assert got[1].isnan().all() and torch.equal(got[keep], K.linear_tiles_fp8(wide[:, :Kd], *qb)[keep])
+    assert K.linear_tiles_fp8(wide[:0, :Kd], *qb).shape == (0, N)
+
+
+def test_linear_fp8_takes_the_same_values_whatever_kernel_takes_it():
+    w = torch.nn.Parameter(rnd(768, 768, seed=2, scale=0.1))
+    x = rnd(9000, 768, seed=1, dtype=BF16)
+    with torch.no_grad():
+        whole = Fn.linear_fp8(x, w)
+        for n in (1, 16, 17, 64, 1000, 4032, 4033, 8999):
+            assert torch.equal(Fn.linear_fp8(x[:n], w), whole[:n]), n
+
+
 def test_linear_fp8_and_its_weight_copy():
     x, w = rnd(2, 5, 300, seed=1, dtype=BF16), torch.nn.Parameter(rnd(140, 300, seed=2, scale=0.1))
     b = rnd(140, seed=3)
