@@ -53,56 +53,75 @@ __device__ __forceinline__ void store_out4(const Fp8Args& p, int m, int n, f32x4
 // ------------------------------------------------------------------------------------------------
 enum { A_F32 = 0, A_BF16 = 1, A_FP8 = 2 };
 
-// Sixteen consecutive columns of a 16- or 32-bit row, of which n exist (the others are zero).  Rows may start on any element.
-template <int AT> struct Sixteen { float v[16]; };
-template <int AT> __device__ __forceinline__ Sixteen<AT> load16(const unsigned char* row, int col, int n) {
-    Sixteen<AT> s;
-    if constexpr (AT == A_BF16) {
-        typedef __attribute__((ext_vector_type(8), aligned(2))) unsigned short us8;
+// Eight consecutive columns of a 16- or 32-bit row as they lie in memory, of which n exist (the others are zero).  Rows may start on
+// any element.  grow(): the running maximum of the magnitudes; amax(): its fp32 bit pattern; pack(h): half h as e4m3.
+template <int AT> struct Eight;
+template <> struct Eight<A_BF16> {
+    typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned V;
+    V v;
+    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
         const bf16_t* p = reinterpret_cast<const bf16_t*>(row) + col;
-        if (n >= 16) {
-            const us8 x = *reinterpret_cast<const us8*>(p), y = *reinterpret_cast<const us8*>(p + 8);
+        v = V{0, 0, 0, 0};
+        if (n >= 8) v = *reinterpret_cast<const V*>(p);
+        else if (n > 0)      // (all loads, then the choice: a load under a condition of its own would wait for the one before)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { s.v[i] = bf2f(x[i]); s.v[8 + i] = bf2f(y[i]); }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s.v[i] = i < n ? bf2f(p[i]) : 0.f;
-        }
-    } else {
-        typedef __attribute__((ext_vector_type(4), aligned(4))) float f4;
-        const float* p = reinterpret_cast<const float*>(row) + col;
-        if (n >= 16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f4 x = reinterpret_cast<const f4*>(p)[i];
-                s.v[4 * i] = x[0]; s.v[4 * i + 1] = x[1]; s.v[4 * i + 2] = x[2]; s.v[4 * i + 3] = x[3];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s.v[i] = i < n ? p[i] : 0.f;
-        }
+            for (int i = 0; i < 7; ++i) { const unsigned e = p[min(i, n - 1)]; v[i >> 1] |= i < n ? e << (i & 1) * 16 : 0; }
     }
-    return s;
-}
+    __device__ __forceinline__ unsigned grow(unsigned m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max_abs_bf16(m, v[i]);
+        return m;
+    }
+    static __device__ __forceinline__ unsigned amax(unsigned m) { return abs_bits_bf16(m); }
+    __device__ __forceinline__ unsigned pack(int h, unsigned byte, bool finite) const {
+        return pack4fp8_bf16(v[2 * h], v[2 * h + 1], scale_value(byte), finite);
+    }
+};
+template <> struct Eight<A_F32> {
+    typedef __attribute__((ext_vector_type(4), aligned(4))) float V;
+    V v[2];
+    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
+        const float* p = reinterpret_cast<const float*>(row) + col;
+        v[0] = v[1] = V{0.f, 0.f, 0.f, 0.f};
+        if (n >= 8) { v[0] = *reinterpret_cast<const V*>(p); v[1] = *reinterpret_cast<const V*>(p + 4); }
+        else if (n > 0)
+#pragma unroll
+            for (int i = 0; i < 7; ++i) { const float e = p[min(i, n - 1)]; v[i >> 2][i & 3] = i < n ? e : 0.f; }
+    }
+    __device__ __forceinline__ unsigned grow(unsigned m) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i >> 2][i & 3]));
+        return m;
+    }
+    static __device__ __forceinline__ unsigned amax(unsigned m) { return m; }
+    __device__ __forceinline__ unsigned pack(int h, unsigned byte, bool finite) const {
+        return pack4fp8(v[h][0], v[h][1], v[h][2], v[h][3], scale_value(byte), finite);
+    }
+};
+template <> struct Eight<A_FP8> {};
+
 // A lane's 32 values of one block of its row, quantised on the way: the block's maximum is the maximum over the four lanes that hold
 // it (16 and 32 apart).  The same values and scale as the row quantiser's.
 template <int AT> __device__ __forceinline__ i32x8 frag_quantised(const unsigned char* row, int kb, int c, int K, unsigned& scale) {
     const int col = kb * 128 + c * 16;
-    const Sixteen<AT> lo = load16<AT>(row, col, K - col), hi = load16<AT>(row, col + 64, K - col - 64);
+    Eight<AT> e[4];
     unsigned m = 0;
+    if (kb * 128 + 128 <= K) {      // (the same for all: no branch per piece but in the last block)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, max(abs_bits(lo.v[i]), abs_bits(hi.v[i])));
+        for (int i = 0; i < 4; ++i) e[i].load(row, col + (i >> 1) * 64 + (i & 1) * 8, 8);
+    } else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i].load(row, col + (i >> 1) * 64 + (i & 1) * 8, K - col - (i >> 1) * 64 - (i & 1) * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = e[i].grow(m);
+    m = Eight<AT>::amax(m);
     m = max(m, (unsigned)__builtin_amdgcn_ds_swizzle((int)m, 0x401f));
     m = max(m, (unsigned)__shfl_xor((int)m, 32, 64));
     scale = scale_byte(m);
-    const float inv = inv_scale(scale);
     const bool finite = m < 0x7f800000u;
     i32x8 f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[i] = (int)pack4fp8(lo.v[4 * i], lo.v[4 * i + 1], lo.v[4 * i + 2], lo.v[4 * i + 3], inv, finite);
-        f[4 + i] = (int)pack4fp8(hi.v[4 * i], hi.v[4 * i + 1], hi.v[4 * i + 2], hi.v[4 * i + 3], inv, finite);
-    }
+    for (int i = 0; i < 8; ++i) f[i] = (int)e[i >> 1].pack(i & 1, scale, finite);
     return f;
 }
 
@@ -199,36 +218,6 @@ template <int AT> struct Tile64 {
     static constexpr int SLOTS = 3, IMAGE = (Q ? 64 : 128) * 128, STAGE = IMAGE + 1024, OPS = Q ? 3 : 5;      // LDS-DMA operations a wave and K-tile
     static constexpr int A_SLOT = 64 * 128 + 256, LDS = SLOTS * STAGE + (Q ? 2 * A_SLOT : 0);
 };
-// eight consecutive columns of a 16- or 32-bit row as they lie in memory, of which n exist (the others are zero)
-template <int AT> struct Eight;
-template <> struct Eight<A_BF16> {
-    typedef __attribute__((ext_vector_type(8), aligned(2))) unsigned short V;
-    V v;
-    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
-        const bf16_t* p = reinterpret_cast<const bf16_t*>(row) + col;
-        v = V{0, 0, 0, 0, 0, 0, 0, 0};
-        if (n >= 8) v = *reinterpret_cast<const V*>(p);
-        else if (n > 0)      // (all loads, then the choice: a load under a condition of its own would wait for the one before)
-#pragma unroll
-            for (int i = 0; i < 7; ++i) { const unsigned short e = p[min(i, n - 1)]; v[i] = i < n ? e : 0; }
-    }
-    __device__ __forceinline__ float at(int i) const { return bf2f(v[i]); }
-};
-template <> struct Eight<A_F32> {
-    typedef __attribute__((ext_vector_type(4), aligned(4))) float V;
-    V v[2];
-    __device__ __forceinline__ void load(const unsigned char* row, int col, int n) {
-        const float* p = reinterpret_cast<const float*>(row) + col;
-        v[0] = v[1] = V{0.f, 0.f, 0.f, 0.f};
-        if (n >= 8) { v[0] = *reinterpret_cast<const V*>(p); v[1] = *reinterpret_cast<const V*>(p + 4); }
-        else if (n > 0)
-#pragma unroll
-            for (int i = 0; i < 7; ++i) { const float e = p[min(i, n - 1)]; v[i >> 2][i & 3] = i < n ? e : 0.f; }
-    }
-    __device__ __forceinline__ float at(int i) const { return v[i >> 2][i & 3]; }
-};
-template <> struct Eight<A_FP8> {};
-
 template <int AT>
 __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws) {
     typedef Tile64<AT> T;
@@ -272,20 +261,17 @@ __global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran,
         if constexpr (Q) {
             unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) m = max(m, abs_bits(raw[i].at(j)));
+            for (int i = 0; i < 4; ++i) m = raw[i].grow(m);
+            m = Eight<AT>::amax(m);
             m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true));      // lanes 1 and 2 apart: the row's four
             m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, true));
             const unsigned byte = scale_byte(m), slot = lds_addr(smem) + T::SLOTS * T::STAGE + (k & 1) * T::A_SLOT;
-            const float inv = inv_scale(byte);
             const bool finite = m < 0x7f800000u;
             // (inline asm: before a write it can see hipcc may wait for the LDS-DMA in flight)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int piece = i * 4 + qpiece;
-                const u32x2 v = {pack4fp8(raw[i].at(0), raw[i].at(1), raw[i].at(2), raw[i].at(3), inv, finite),
-                                 pack4fp8(raw[i].at(4), raw[i].at(5), raw[i].at(6), raw[i].at(7), inv, finite)};
+                const u32x2 v = {raw[i].pack(0, byte, finite), raw[i].pack(1, byte, finite)};
                 asm volatile("ds_write_b64 %0, %1" ::"v"(slot + qrow * 128 + (((piece >> 1) ^ ((qrow >> 1) & 7)) << 4) + (piece & 1) * 8), "v"(v) : "memory");
             }
             if (qpiece == 0) asm volatile("ds_write_b32 %0, %1" ::"v"(slot + 64 * 128 + qrow * 4), "v"(byte) : "memory");

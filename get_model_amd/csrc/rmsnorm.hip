@@ -167,7 +167,7 @@ __global__ __launch_bounds__(1024) void rms_fwd_kernel(FwdArgs p) {
                 const unsigned byte = scale_byte(amax);
                 if (on && col[v] < (int)p.ldq) {      // columns D .. ldq-1 are zeros: padding up to whole blocks
                     *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(p.y) + (size_t)row * p.ldq + col[v]) =
-                        pack4fp8(y.x, y.y, y.z, y.w, inv_scale(byte), amax < 0x7f800000u);
+                        pack4fp8(y.x, y.y, y.z, y.w, scale_value(byte), amax < 0x7f800000u);
                     if ((lane & 31) == 0) p.scales[(size_t)row * p.lds + (col[v] >> 7)] = (unsigned char)byte;
                 }
             } else {
@@ -283,10 +283,10 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t
     __syncthreads();
     m = max(max(red[0], red[1]), max(red[2], red[3]));
     const unsigned byte = scale_byte(m);
-    const float inv = inv_scale(byte);
+    const float scale = scale_value(byte);
     for (int r = r0; r < r1; r += 8) {
         const float4 v = load4<WT>(w, (size_t)r * ldw + c, n);
-        *reinterpret_cast<unsigned*>(q + (size_t)r * ldq + c) = pack4fp8(v.x, v.y, v.z, v.w, inv, m < 0x7f800000u);
+        *reinterpret_cast<unsigned*>(q + (size_t)r * ldq + c) = pack4fp8(v.x, v.y, v.z, v.w, scale, m < 0x7f800000u);
     }
     if (threadIdx.x == 0) scales[(size_t)blockIdx.y * lds + blockIdx.x] = (unsigned char)byte;
 }
