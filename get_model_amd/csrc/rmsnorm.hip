@@ -262,8 +262,7 @@ __global__ __launch_bounds__(1024) void rms_bwd_kernel(BwdArgs p) {
     }
 }
 
-// weight[N, K] -> e4m3 [N, ldq] and one scale per 128 x 128 block: one workgroup per block; rows in two passes over the
-// block (the second one comes out of the cache)
+// weight[N, K] -> e4m3 [N, ldq] and one scale per 128 x 128 block: one workgroup per block, 64 values a thread in registers
 template <int WT>
 __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t ldw, unsigned char* q, size_t ldq, unsigned char* scales,
                                                            int lds, int N, int K) {
@@ -271,10 +270,13 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * 128 + (lane & 31) * 4, n = K - c;
     const int r0 = blockIdx.y * 128 + wave * 2 + (lane >> 5);
-    const int r1 = min(N, (int)(blockIdx.y + 1) * 128);
+    typename Raw<WT>::type raw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) raw[i] = load_raw<WT, false>(w, (size_t)(r0 + 8 * i) * ldw + c, r0 + 8 * i < N ? n : 0);
     unsigned m = 0;
-    for (int r = r0; r < r1; r += 8) {
-        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float4 v = widen(raw[i]);
         m = max(m, max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w))));
     }
     m = max32(m);
@@ -284,9 +286,11 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const void* w, size_t
     m = max(max(red[0], red[1]), max(red[2], red[3]));
     const unsigned byte = scale_byte(m);
     const float scale = scale_value(byte);
-    for (int r = r0; r < r1; r += 8) {
-        const float4 v = load4<WT>(w, (size_t)r * ldw + c, n);
-        *reinterpret_cast<unsigned*>(q + (size_t)r * ldq + c) = pack4fp8(v.x, v.y, v.z, v.w, scale, m < 0x7f800000u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float4 v = widen(raw[i]);
+        if (r0 + 8 * i < N)
+            *reinterpret_cast<unsigned*>(q + (size_t)(r0 + 8 * i) * ldq + c) = pack4fp8(v.x, v.y, v.z, v.w, scale, m < 0x7f800000u);
     }
     if (threadIdx.x == 0) scales[(size_t)blockIdx.y * lds + blockIdx.x] = (unsigned char)byte;
 }

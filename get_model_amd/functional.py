@@ -945,10 +945,10 @@ def linear_fp8(x, weight, bias=None):
     if pair:
         return K.gemm_fp8(x[0], x[1], qw, sw, bias)
     rows = _flat(x, x.shape[-1])
-    # Few rows, no large weight: quantised inside the product, one launch instead of two (1 x 768 x 768 15.0 -> 8.4 us, 16 x 4096 x 4096
-    # 14.5 -> 8.7); with a large one every workgroup's own quantisation costs more than the launch (8192 x 8192: 16.8 -> 22.5).
-    # More rows: the same in 64 x 64 tiles, while they are few and the depth is short (201 x 2304 x 768 15.3 -> 7.9, 4020 x 768 x 768 15.6
-    # -> 12.9; but 2010 x 2304 x 768 15.6 -> 19.5, 201 x 768 x 3000 15.3 -> 23.9).
+    # Few rows, no large weight: quantised inside the product, one launch instead of two (1 x 768 x 768 14.9 -> 8.3 us, 16 x 4096 x 4096
+    # 15.1 -> 8.1); with a large one every workgroup's own quantisation costs more than the launch (16 x 8192 x 8192: 20.2 -> 24.5).
+    # More rows: the same in 64 x 64 tiles, while they are few and the depth is short (201 x 2304 x 768 14.3 -> 6.9, 4020 x 768 x 768 14.3
+    # -> 11.0; but 2010 x 2304 x 768 15.4 -> 17.1, 201 x 768 x 3000 14.1 -> 21.3).
     M, depth = rows.shape[0], qw.shape[1] >> 7
     if M <= 16 and qw.numel() <= 1 << 25:
         out = K.linear_rows_fp8(rows, qw, sw, bias)
