@@ -206,27 +206,37 @@ template <int N> __device__ __forceinline__ void wait_vm() {
 // CU.  The scale words (64 rows of A, then the tile's one block of B) ride in a 1-KiB slot beside each K-tile.  What bounds it is
 // the CU's path to the caches (16 KiB a K-tile at about 24 bytes a clock), not the depth of the ring: rings of 2, 4 and 6 and tiles
 // of 128 x 64, 64 x 128, 128 x 128, 64 x 32, 32 x 64 and 32 x 32 measured within 10 % or slower over 28 shapes (4020 x 768 x 768:
-// 8.6 us host-bound, 1000 x 2304 x 2304: 15.4).  splits > 1: workgroup (tile, s) takes the s-th part of the depth.
+// 8.4 us, 1000 x 2304 x 2304: 14.6).  Tiles of 128 x 128 whose LDS reads run under the products gain only where 128 to 256 of them fill the
+// chip just once (1024 x 4096 x 4096 29 us against 36; 2048 x 2304 x 2304 30 against 23), with two workgroups a CU the other way round
+// (30 and 20.6): not kept.  splits > 1: workgroup (tile, s) takes the s-th part of the depth.
 //
 // AT: e4m3 rows, or 16- / 32-bit rows (p.sa unused, p.lda in bytes, p.Ka columns) that are quantised on their way into LDS: four
 // threads a row, their pieces of 8 columns side by side, loaded a K-tile ahead; two slots of A's image and scales behind B's ring.
 // A K-tile takes 0.78 us there, what its steps take one behind the other, or 1.8 ns x tiles; GPU time of 201 x 768 x 768 6.6 us, with the
 // row quantiser before the product 6.9.  Loads two K-tiles ahead measured the same (hipcc waits for all loads when LDS-DMA is in flight).
 // ------------------------------------------------------------------------------------------------
+// Tile number lid: groups of `group` columns of tiles one after the other, row by row inside a group (see group_of).
+__device__ __forceinline__ void tile_of(int lid, int tiles_m, int tiles_n, int group, int& tm, int& tn) {
+    const int per = tiles_m * group, g = lid / per, rem = lid - g * per, w = min(group, tiles_n - g * group);
+    tm = rem / w;
+    tn = g * group + (rem - tm * w);
+}
 template <int AT> struct Tile64 {
     static constexpr bool Q = AT != A_FP8;
     static constexpr int SLOTS = 3, IMAGE = (Q ? 64 : 128) * 128, STAGE = IMAGE + 1024, OPS = Q ? 3 : 5;      // LDS-DMA operations a wave and K-tile
     static constexpr int A_SLOT = 64 * 128 + 256, LDS = SLOTS * STAGE + (Q ? 2 * A_SLOT : 0);
 };
 template <int AT>
-__global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws) {
+__global__ __launch_bounds__(256) void gemm_fp8_tile_kernel(Fp8Args p, int gran, int splits, float* ws, int group) {
     typedef Tile64<AT> T;
     constexpr bool Q = T::Q;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1, nkb = p.K >> 7;
-    const int tiles_n = (p.N + 63) / 64, bid = xcd_remap(blockIdx.x, gridDim.x), lid = bid / splits, sp = bid - lid * splits;
-    const int tm = lid / tiles_n, tn = lid - tm * tiles_n, m0 = tm * 64, n0 = tn * 64;
+    const int bid = xcd_remap(blockIdx.x, gridDim.x), lid = bid / splits, sp = bid - lid * splits;
+    int tm, tn;
+    tile_of(lid, (p.M + 63) / 64, (p.N + 63) / 64, group, tm, tn);
+    const int m0 = tm * 64, n0 = tn * 64;
     const int kb0 = (int)((int64_t)nkb * sp / splits), nk = (int)((int64_t)nkb * (sp + 1) / splits) - kb0;      // >= 1: splits <= nkb
     // 16-byte pieces: wave w's i-th instruction moves rows 8 (4 i + w) .. + 7 of the [A; B] image
     const unsigned char* src[4];
@@ -717,10 +727,23 @@ template <int MT, int NT, int AT = A_FP8> static int launch_rows(const Fp8Args& 
     GETMI_CHECK_LAUNCH("gemm_fp8");
     return GETMI_OK;
 }
+// Columns of 64 x 64 tiles in a group: the tiles that run at once on an XCD (3 on each of 32 CUs) make a square of the output, so that
+// its L2 fetches the fewest rows of both operands.  Against whole rows of tiles: 1024 x 4096 x 4096 43 -> 36 us, 256 x 8192 x 8192 41.6 ->
+// 35.6, 400 x 3000 x 3000 15.4 -> 12.7.
+static int group_of(int M, int N, int splits) {
+    const int tm = (M + 63) / 64, tn = (N + 63) / 64;
+    int64_t t = ((int64_t)tm * tn + 7) / 8;
+    if (t > 96 / splits) t = 96 / splits;
+    int g = 1;
+    while (g * g < t) ++g;
+    if ((int64_t)g * tm < t) g = (int)((t + tm - 1) / tm);
+    return g < tn ? g : tn;
+}
 template <int AT = A_FP8> static int launch_tile(const Fp8Args& p, int gran, int splits, float* ws, hipStream_t st) {
     const int64_t tiles = (int64_t)((p.M + 63) / 64) * ((p.N + 63) / 64);
     GETMI_CHECK_ARG(tiles * splits < 1 << 24, "gemm_fp8: M=%d N=%d too large", p.M, p.N);      // a launch is at most 2^32 - 1 threads wide
-    hipLaunchKernelGGL(gemm_fp8_tile_kernel<AT>, dim3((unsigned)(tiles * splits)), dim3(256), Tile64<AT>::LDS, st, p, gran, splits, ws);
+    hipLaunchKernelGGL(gemm_fp8_tile_kernel<AT>, dim3((unsigned)(tiles * splits)), dim3(256), Tile64<AT>::LDS, st, p, gran, splits, ws,
+                       group_of(p.M, p.N, splits));
     if (splits > 1) {
         const int64_t blocks = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
         hipLaunchKernelGGL(gemm_fp8_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p, gran, splits,
@@ -772,7 +795,7 @@ template <int GR> static int launch_big(const Fp8Args& p, int gran, hipStream_t 
 //   up to 16 rows    rows kernel: 1 x 8192 x 8192 13.6 (4.9 TB/s) against 64-row tiles 22.5; 8 x 768 x 8192 9.0 against 21.7.  Two
 //                    16-row groups of B a workgroup where both sides are wide (16 x 8192 x 8192 20.0 -> 17.2; 1 row: 13.6 -> 16.6)
 //   up to 32, N <= 4096   rows kernel with two row groups: 8 x 768 x 8192 9.8; at N = 8192 64-row tiles in two splits win, 22 -> 15.6
-//   64 x 64 tiles    a K-tile costs a CU 16 KiB of its one path to the caches (1.1 ns x tiles over the chip), a lone workgroup 0.34 us
+//   64 x 64 tiles    a K-tile costs a CU 16 KiB of its one path to the caches (1.0 - 1.2 ns x tiles over the chip), a lone workgroup 0.34 us
 //   256 x 256 tiles  1.15 us a K-tile with few CUs busy, 1.85 with all (the same path: 64 KiB), 3.5 for the tile's ends
 //                    4020 x 768 x 768 8.6 against 12.2, 12060 x 768 x 768 18.3 against 13.3, 2000 x 4096 x 4096 76 against 39
 //   depth of 6144 on and few 64-row tiles: the depth is split and joined by a second kernel (64 x 8192 x 8192 23.5 -> 17.1,
